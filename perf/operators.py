@@ -143,7 +143,7 @@ def prepare(case, seed):
         s["corpus"] = c
         if case["op"] == "log_probs":
             k, given = case["k"], case["given"]
-            c.reserve_log_probs(nq, k=k, source=_source(case))
+            c.reserve_log_probs(nq, source=_source(case))
             s["lp"] = torch.empty(nq, given, device="cuda")
             s["lse"] = torch.empty(nq, device="cuda")
             s["entropy"] = torch.empty(nq, device="cuda")
