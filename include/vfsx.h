@@ -441,6 +441,70 @@ int vfsx_corpus_scan_time_ms(vfsx_corpus *c, double *total_ms, uint64_t *launche
  * VFSX_EUCLIDEAN_I8DOMAIN serve k <= 1024. */
 #define VFSX_MAX_K (1u << 20)
 
+/* ---- probabilities over the store (no reference counterpart) ----------------------------------------------------
+ *
+ * A search says which rows are nearest; these entry points say with what probability, under the softmax over the whole
+ * store (the confidence of a retrieval; or the rows are a model's output table, one row per token, and the queries its
+ * hidden states):
+ *   logit    l_j = sim(q, x_j) / temperature + bias_j
+ *   lse      log sum_j exp(l_j)
+ *   log p_j  = l_j - lse,   entropy = -sum_j p_j log p_j  (natural logarithms)
+ * Rows are the store's values (f32; int8 rows v as v / scale, with the quotient taken once per product), or those of the 8-bit
+ * floating point copy below.  A row with bias -inf is not there: probability 0.  VFSX_SIM_COSINE divides by both norms; a row or
+ * query whose squared norm is 0 in f32 has no cosine: that row is not there, for that query no row is.
+ * When no row is there (an empty store, everything masked): lse = -inf, entropy = 0, log probabilities -inf, no top rows.
+ * A logit that is NaN or infinite in f32 makes all results of its query NaN, and its top rows empty (flags = 0).
+ */
+typedef enum vfsx_similarity { VFSX_SIM_DOT = 0, VFSX_SIM_COSINE = 1 } vfsx_similarity;
+typedef enum vfsx_source { VFSX_SOURCE_ROWS = 0, VFSX_SOURCE_F8 = 1 } vfsx_source;
+#define VFSX_LOG_PROBS_MAX_K 128
+
+/*
+ * For each of nq queries (device, f32, row-major), enqueued on `stream` without host synchronisation:
+ *   d_bias       [rows of the store] f32 added to the logits, or NULL
+ *   d_rows       [nq][n_given] global scan positions (row_base + local row) whose log probabilities are wanted; a position the
+ *                store does not hold (~0 for an unused place) has log probability -inf
+ *   d_log_probs  [nq][n_given];   d_lse [nq], d_entropy [nq]: may be NULL
+ *   d_top        [nq][k] vfsx_hit, the k most probable rows by (logit descending, row ascending), `dist` = log probability; places
+ *                beyond the rows there are have flags = 0, row = id = ~0, dist = -inf.  k <= VFSX_LOG_PROBS_MAX_K, 0 = none
+ * The order of the top rows is that of logits computed in 64 bits.  On a row-sharded store the results are this shard's:
+ * log p over all shards is log p + lse - log sum_shards exp(lse).
+ * Calls on one corpus share its workspaces, as searches do (see vfsx_search_device).  Under HIP graph capture the call makes no
+ * allocation: call vfsx_reserve_log_probs with at least these sizes first (VFSX_ERR_MEMTABLE otherwise); memory a captured
+ * call used stays until the corpus is destroyed, the graph is valid until rows are appended, and a replay counts as a call: replays
+ * and calls on one corpus must not overlap.
+ */
+int vfsx_log_probs_device(vfsx_corpus *c, const float *d_queries, uint32_t nq, int similarity, double temperature, int source,
+                          const float *d_bias, const uint64_t *d_rows, uint32_t n_given, uint32_t k, float *d_log_probs,
+                          float *d_lse, float *d_entropy, vfsx_hit *d_top, void *stream);
+/* The same with host buffers (bias included); returns when the results are there. */
+int vfsx_log_probs(vfsx_corpus *c, const float *queries, uint32_t nq, int similarity, double temperature, int source,
+                   const float *bias, const uint64_t *rows, uint32_t n_given, uint32_t k, float *log_probs, float *lse,
+                   float *entropy, vfsx_hit *top);
+/* Builds what vfsx_log_probs keeps per row and allocates its workspaces for calls of up to nq queries. */
+int vfsx_reserve_log_probs(vfsx_corpus *c, uint32_t nq, int source);
+
+/* ---- 8-bit floating point copy of an f32 store and its product with queries (no reference counterpart) ----------------
+ *
+ * enable != 0 keeps a copy of the rows in e4m3 (1 byte per element, +1/128 for the scales) beside the f32 rows, extended when
+ * rows are appended: elements 128 kb .. 128 kb + 127 of a row share one scale 2^e, e the least integer >= -127 with
+ * max|x| <= 448 * 2^e, values rounded to nearest even.  Queries are converted by the same rule in the call.  (A block holding a NaN
+ * or an infinity becomes NaN.)  Searches do not use it.  0 frees it.  int8 stores are refused: they are 8 bits wide already.
+ */
+int vfsx_corpus_enable_f8(vfsx_corpus *c, int enable);
+/* The values the copy holds for LOCAL rows, as f32 (exact; the one value above the f32 range, 2^128, as infinity), row-major. */
+int vfsx_corpus_get_rows_f8(vfsx_corpus *c, const uint64_t *rows, uint64_t n, float *out);
+typedef enum vfsx_scores_dtype { VFSX_SCORES_F32 = 0, VFSX_SCORES_BF16 = 1 } vfsx_scores_dtype;
+/*
+ * All scores: out[q][j] = q8 . x8_j (VFSX_SIM_DOT), divided by the norms of the f32 query and row (VFSX_SIM_COSINE; NaN where
+ * one of them has none).  out is [nq][ld] f32 or bf16 with ld >= rows (0 = rows; elements beyond the rows are not written).
+ * Accumulated in f32, rounded once.  Capture and workspaces as above (vfsx_reserve_scores_f8).
+ */
+int vfsx_scores_f8_device(vfsx_corpus *c, const float *d_queries, uint32_t nq, int similarity, int out_dtype, void *d_out,
+                          uint64_t ld, void *stream);
+int vfsx_scores_f8(vfsx_corpus *c, const float *queries, uint32_t nq, int similarity, int out_dtype, void *out, uint64_t ld);
+int vfsx_reserve_scores_f8(vfsx_corpus *c, uint32_t nq);
+
 #ifdef __cplusplus
 }
 #endif

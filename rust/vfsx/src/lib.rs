@@ -71,6 +71,15 @@ extern "C" {
     pub fn vfsx_corpus_load_log(c: *mut VfsxCorpus, path: *const c_char, n_loaded: *mut u64) -> c_int;
     pub fn vfsx_corpus_load_log_range(c: *mut VfsxCorpus, path: *const c_char, first_record: u64, max_records: u64, n_loaded: *mut u64) -> c_int;
     pub fn vfsx_corpus_get_metadata_json(c: *mut VfsxCorpus, row: u64, buf: *mut c_char, cap: u64, needed: *mut u64) -> c_int;
+    // ---- probabilities over the store, 8-bit floating point copy
+    pub fn vfsx_log_probs_device(c: *mut VfsxCorpus, d_queries: *const f32, nq: u32, similarity: c_int, temperature: f64, source: c_int, d_bias: *const f32, d_rows: *const u64, n_given: u32, k: u32, d_log_probs: *mut f32, d_lse: *mut f32, d_entropy: *mut f32, d_top: *mut VfsxHit, stream: *mut c_void) -> c_int;
+    pub fn vfsx_log_probs(c: *mut VfsxCorpus, queries: *const f32, nq: u32, similarity: c_int, temperature: f64, source: c_int, bias: *const f32, rows: *const u64, n_given: u32, k: u32, log_probs: *mut f32, lse: *mut f32, entropy: *mut f32, top: *mut VfsxHit) -> c_int;
+    pub fn vfsx_reserve_log_probs(c: *mut VfsxCorpus, nq: u32, source: c_int) -> c_int;
+    pub fn vfsx_corpus_enable_f8(c: *mut VfsxCorpus, enable: c_int) -> c_int;
+    pub fn vfsx_corpus_get_rows_f8(c: *mut VfsxCorpus, rows: *const u64, n: u64, out: *mut f32) -> c_int;
+    pub fn vfsx_scores_f8_device(c: *mut VfsxCorpus, d_queries: *const f32, nq: u32, similarity: c_int, out_dtype: c_int, d_out: *mut c_void, ld: u64, stream: *mut c_void) -> c_int;
+    pub fn vfsx_scores_f8(c: *mut VfsxCorpus, queries: *const f32, nq: u32, similarity: c_int, out_dtype: c_int, out: *mut c_void, ld: u64) -> c_int;
+    pub fn vfsx_reserve_scores_f8(c: *mut VfsxCorpus, nq: u32) -> c_int;
     // ---- search
     pub fn vfsx_search(c: *mut VfsxCorpus, queries: *const f32, nq: u32, k: u32, metric: c_int, out_ids: *mut u64, out_dist: *mut f32, out_count: *mut u32) -> c_int;
     pub fn vfsx_search_device(c: *mut VfsxCorpus, d_queries: *const f32, nq: u32, k: u32, metric: c_int, d_hits: *mut VfsxHit, stream: *mut c_void) -> c_int;
@@ -292,6 +301,26 @@ impl Corpus {
     /// Benchmark utility: counter-based synthetic rows generated on the device.
     pub fn fill_synthetic(&mut self, seed: u64, row0: u64, n: u64, id0: u64) -> io::Result<()> {
         check(unsafe { vfsx_corpus_fill_synthetic(self.h, seed, row0, n, id0) })
+    }
+
+    /// Log probabilities of the hits of a search: `rows[nq][given]` global scan positions under the softmax of
+    /// cosine(query, row) / temperature over the whole store, and the entropy per query.
+    pub fn log_probs_cosine(&mut self, queries: &[f32], rows: &[u64], temperature: f64) -> io::Result<(Vec<f32>, Vec<f32>)> {
+        if self.dim == 0 || queries.len() % self.dim != 0 {
+            return Err(io::Error::new(io::ErrorKind::InvalidInput, "queries must be a whole number of vectors"));
+        }
+        let nq = queries.len() / self.dim;
+        if nq == 0 {
+            return Ok((Vec::new(), Vec::new()));
+        }
+        if rows.len() % nq != 0 {
+            return Err(io::Error::new(io::ErrorKind::InvalidInput, "rows must be the same number for every query"));
+        }
+        let (mut lp, mut entropy) = (vec![0f32; rows.len()], vec![0f32; nq]);
+        check(unsafe {
+            vfsx_log_probs(self.h, queries.as_ptr(), nq as u32, 1, temperature, 0, std::ptr::null(), rows.as_ptr(), (rows.len() / nq) as u32, 0, lp.as_mut_ptr(), std::ptr::null_mut(), entropy.as_mut_ptr(), std::ptr::null_mut())
+        })?;
+        Ok((lp, entropy))
     }
 
     /// `nq` queries at once ("A2/A3 + A4 per query"): flat `[nq][k]` ids / distances and per-query counts.

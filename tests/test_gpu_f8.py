@@ -1,0 +1,194 @@
+"""GPU: the 8-bit floating point copy of a store and the product with it, against their definition in 64 bits."""
+import numpy as np
+import pytest
+
+import vfs_amd
+from vfs_amd import _lib
+from tests import prob_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def make(n, d, rng):
+    return (rng.standard_normal((n, d)) / np.sqrt(d) * np.exp(rng.standard_normal((n, 1)))).astype(np.float32)
+
+
+def f8_corpus(rows, **kw):
+    c = vfs_amd.Corpus(rows.shape[1], **kw)
+    if len(rows):
+        c.append(rows)
+    c.enable_f8()
+    return c
+
+
+@pytest.mark.parametrize("n,d", [(1, 1), (3, 5), (64, 127), (65, 128), (130, 129), (300, 511), (257, 512), (40, 640), (1000, 777)])
+def test_copy_holds_what_the_rule_says(n, d):
+    rng = np.random.default_rng(n + d)
+    x = (make(n, d, rng) * 2.0 ** rng.integers(-20, 20, (n, 1))).astype(np.float32)
+    x[0, 0] = 448.0
+    x[-1, -1] = np.nextafter(np.float32(448.0), np.float32(1e9))
+    c = f8_corpus(x)
+    assert np.array_equal(c.get_rows_f8(np.arange(n)).astype(np.float64), ref.e4m3_values(x))
+
+
+def test_copy_at_the_ends_of_f32():
+    x = np.zeros((12, 256), np.float32)
+    x[1, :5] = [2.0**-149, 2.0**-140, 2.0**-130, -2.0**-149, 0]
+    x[2, 200] = np.finfo(np.float32).max
+    x[3, :128] = 2.0**-126
+    x[4, 3], x[5, 130], x[6, 0] = np.nan, np.inf, -np.inf
+    x[7] = np.float32(1.0) + np.arange(256, dtype=np.float32) / 256  # halves between e4m3 values: ties to even
+    x[8] = np.float32(2.0**-7) * np.arange(256, dtype=np.float32)
+    x[8, 0] = x[8, 128] = 448.0                                     # scale 1: steps of 2^-9 below 2^-6
+    x[9, :128] = -0.0
+    c = f8_corpus(x)
+    # (the largest f32 rounds up to 256 * 2^120 = 2^128 in the copy, which as an f32 is infinity)
+    with np.errstate(over="ignore"):
+        got, want = c.get_rows_f8(np.arange(12)), ref.e4m3_values(x).astype(np.float32)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isnan(want).sum() == 3 * 128
+    assert np.array_equal(got[~np.isnan(want)], want[~np.isnan(want)])
+
+
+def score_bound(rows, q):
+    """Products of e4m3 values are exact; d of them accumulated in f32, in any order and aligned to the largest before they are
+    added (2^-23 a step): (d + 64) 2^-23 sum |q8 x8|."""
+    a, b = np.abs(ref.e4m3_values(q)), np.abs(ref.e4m3_values(rows))
+    return (rows.shape[1] + 64) * 2.0**-23 * (a @ b.T)
+
+
+SIZES = [(1, 1, 1), (2, 3, 2), (31, 16, 1), (32, 64, 3), (33, 127, 5), (64, 128, 16), (65, 129, 17), (128, 200, 33), (255, 256, 64), (257, 300, 65),
+         (1000, 96, 2), (1003, 777, 37), (5000, 130, 130), (300, 512, 300), (700, 2050, 1), (513, 1024, 257), (40000, 33, 4)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("similarity", ["dot", "cosine"])
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_scores_against_definition(size, similarity, dtype):
+    import torch
+    n, d, nq = size
+    rng = np.random.default_rng(n * 3 + d)
+    rows, q = make(n, d, rng), (rng.standard_normal((nq, d)) * np.exp(rng.standard_normal((nq, 1)))).astype(np.float32)
+    c = f8_corpus(rows)
+    want, tol = ref.e4m3_values(q) @ ref.e4m3_values(rows).T, score_bound(rows, q)
+    if similarity == "cosine":
+        by = np.linalg.norm(q.astype(np.float64), axis=1)[:, None] * np.linalg.norm(rows.astype(np.float64), axis=1)[None, :]
+        want, tol = want / by, tol / by + 3 * 2.0**-24 * np.abs(want / by)
+    ld = n + (n % 3) * 5  # rows of the output may be longer
+    out = torch.full((nq + 1, ld), 7.0, device="cuda", dtype=torch.float32 if dtype == "f32" else torch.bfloat16)
+    qd = torch.from_numpy(q).cuda()
+    c.scores_f8_device(qd.data_ptr(), nq, out.data_ptr(), ld=ld, dtype=dtype, similarity=similarity, stream=torch.cuda.current_stream().cuda_stream)
+    got = out.double().cpu().numpy()
+    half = 2.0**-24 if dtype == "f32" else 2.0**-8
+    err = np.abs(got[:nq, :n] - want) - (tol * (1 + half) + half * np.abs(want))
+    assert (err <= 0).all(), err.max()
+    assert (got[nq] == 7).all() and (got[:, n:] == 7).all()  # what is not the call's stays
+    if dtype == "f32":
+        assert np.array_equal(c.scores_f8(q, similarity), got[:nq, :n].astype(np.float32))
+
+
+def test_scores_of_odd_values():
+    rng = np.random.default_rng(1)
+    rows, q = make(100, 140, rng), rng.standard_normal((34, 140)).astype(np.float32)
+    rows[3] = 0
+    rows[7, 139], rows[9, 0] = np.nan, np.inf
+    q[2] = 0
+    q[5, 6] = np.nan
+    for nq in (6, 34):
+        c = f8_corpus(rows)
+        dot, cos = c.scores_f8(q[:nq]), c.scores_f8(q[:nq], "cosine")
+        bad = np.zeros((nq, 100), bool)
+        bad[:, [7, 9]] = bad[5] = True
+        assert np.array_equal(np.isnan(dot), bad) and (dot[~bad[:, 3], 3] == 0).all() and (dot[2][~bad[2]] == 0).all()
+        bad[:, 3] = bad[2] = True  # no cosine
+        assert np.array_equal(np.isnan(cos), bad)
+
+
+def test_small_and_large_scales():
+    """Scales far from 1 on both sides: their product may leave the range of one e8m0 scale."""
+    rng = np.random.default_rng(2)
+    rows = (make(90, 300, rng) * 2.0 ** rng.integers(-100, 100, (90, 1))).astype(np.float32)
+    q = (rng.standard_normal((40, 300)) * 2.0 ** rng.integers(-20, 20, (40, 1))).astype(np.float32)
+    c = f8_corpus(rows)
+    want, tol = ref.e4m3_values(q) @ ref.e4m3_values(rows).T, score_bound(rows, q)
+    for nq in (1, 40):
+        got = c.scores_f8(q[:nq]).astype(np.float64)
+        assert (np.abs(got - want[:nq]) <= tol[:nq] + 2.0**-24 * np.abs(want[:nq]) + 2.0**-148).all()
+    # elements of very different size in one row: the blocks of 128 have scales of their own
+    rows = make(50, 512, rng)
+    rows[:, 128:256] *= 2.0**60
+    rows[:, 300] *= 2.0**-50
+    q = rng.standard_normal((33, 512)).astype(np.float32)
+    q[:, 128:256] *= np.float32(2.0**-60)
+    got = f8_corpus(rows).scores_f8(q).astype(np.float64)
+    want, tol = ref.e4m3_values(q) @ ref.e4m3_values(rows).T, score_bound(rows, q)
+    assert (np.abs(got - want) <= tol + 2.0**-24 * np.abs(want)).all()
+
+
+def test_copy_follows_appends_and_can_be_switched():
+    rng = np.random.default_rng(3)
+    rows, q = make(900, 150, rng), rng.standard_normal((3, 150)).astype(np.float32)
+    c = f8_corpus(rows[:0])
+    assert c.scores_f8(q).shape == (3, 0)
+    c.set_insert_batch(32)
+    at = 0
+    for more in (1, 62, 3, 200, 16, 618):
+        c.append(rows[at:at + more])
+        at += more
+        assert np.array_equal(c.scores_f8(q), f8_corpus(rows[:at]).scores_f8(q))
+    assert np.array_equal(c.get_rows_f8(np.arange(900)).astype(np.float64), ref.e4m3_values(rows))
+    before = c.storage_info()["device_bytes"]
+    c.enable_f8(False)
+    assert c.storage_info()["device_bytes"] < before
+    for call in (lambda: c.scores_f8(q), lambda: c.get_rows_f8([0]), lambda: c.log_probs(q, source="f8"), lambda: c.reserve_scores_f8(1),
+                 lambda: c.reserve_log_probs(1, source="f8")):
+        with pytest.raises(vfs_amd.VfsxError) as e:
+            call()
+        assert e.value.code == _lib.ERR_INVALID_VECTOR and "enable_f8" in str(e.value)
+    c.enable_f8()
+    assert np.array_equal(c.scores_f8(q), f8_corpus(rows).scores_f8(q))
+
+
+def test_refusals():
+    rng = np.random.default_rng(4)
+    c, q = f8_corpus(make(20, 8, rng)), np.ones((2, 8), np.float32)
+    with pytest.raises(vfs_amd.VfsxError):
+        vfs_amd.Corpus(8, quantize=True).enable_f8()
+    with pytest.raises(vfs_amd.VfsxError):
+        c.scores_f8(np.ones((2, 9), np.float32))
+    with pytest.raises(vfs_amd.VfsxError):
+        c.scores_f8(q, "euclid")
+    with pytest.raises(vfs_amd.VfsxError):
+        c.get_rows_f8([20])
+    out = np.zeros((2, 20), np.float32)
+    lib, bad = c._lib, _lib.ERR_INVALID_VECTOR
+    assert lib.vfsx_scores_f8(c.handle, q.ctypes.data, 2, 0, 0, out.ctypes.data, 19) == bad   # rows shorter than the store
+    assert lib.vfsx_scores_f8(c.handle, q.ctypes.data, 2, 0, 2, out.ctypes.data, 0) == bad
+    assert lib.vfsx_scores_f8(c.handle, None, 2, 0, 0, out.ctypes.data, 0) == bad
+    assert lib.vfsx_scores_f8(c.handle, q.ctypes.data, 2, 0, 0, None, 0) == bad
+    assert lib.vfsx_scores_f8(c.handle, None, 0, 0, 0, None, 0) == 0
+    assert c.scores_f8(q).shape == (2, 20)
+
+
+def test_captured_graph():
+    import torch
+    rng = np.random.default_rng(5)
+    c = f8_corpus(make(700, 300, rng))
+    q, out = torch.zeros(40, 300, device="cuda"), torch.zeros(40, 700, device="cuda", dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+    c.reserve_scores_f8(40)
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+        c.scores_f8_device(q.data_ptr(), 40, out.data_ptr(), dtype="bf16", stream=side.cuda_stream)
+    for turn in range(4):
+        q.copy_(torch.from_numpy(rng.standard_normal((40, 300)).astype(np.float32)))
+        out.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        eager = torch.zeros_like(out)
+        c.scores_f8_device(q.data_ptr(), 40, eager.data_ptr(), dtype="bf16", stream=torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and bool((out != 0).any())
+        if turn == 1:
+            c.scores_f8(rng.standard_normal((3000, 300)).astype(np.float32))  # a larger call replaces the workspace

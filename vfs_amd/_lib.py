@@ -19,6 +19,10 @@ ERR_INTERNAL = -6
 ERR_NO_DEVICE = -7
 
 F32, I8 = 0, 1
+SIMILARITY = {"dot": 0, "cosine": 1}           # vfsx_similarity
+SOURCE = {"rows": 0, "f8": 1}                  # vfsx_source
+SCORES_DTYPE = {"f32": 0, "bf16": 1}           # vfsx_scores_dtype
+LOG_PROBS_MAX_K = 128                          # VFSX_LOG_PROBS_MAX_K
 MAX_K = 1 << 20  # VFSX_MAX_K; results beyond 128 hits: one scan + a radix select over every row's key
 
 # every symbol include/vfsx.h declares
@@ -35,6 +39,8 @@ SYMBOLS = (
     "vfsx_comm_rccl_version", "vfsx_search_sharded", "vfsx_search_sharded_host", "vfsx_comm_merge_hits",
     "vfsx_comm_reserve", "vfsx_comm_alloc_count", "vfsx_corpus_storage_info",
     "vfsx_corpus_set_insert_batch", "vfsx_corpus_commit", "vfsx_quantize_rows_host",
+    "vfsx_log_probs", "vfsx_log_probs_device", "vfsx_reserve_log_probs", "vfsx_corpus_enable_f8", "vfsx_corpus_get_rows_f8",
+    "vfsx_scores_f8", "vfsx_scores_f8_device", "vfsx_reserve_scores_f8",
 )
 COMM_ID_BYTES = 128
 
@@ -137,6 +143,15 @@ def load() -> C.CDLL:
     lib.vfsx_search_sharded.argtypes = [vp, vp, vp, C.c_uint32, C.c_uint32, C.c_int, vp, vp]
     lib.vfsx_comm_merge_hits.argtypes = [vp, vp, C.c_uint32, C.c_uint32, vp, vp]
     lib.vfsx_search_sharded_host.argtypes = [vp, vp, f32p, C.c_uint32, C.c_uint32, C.c_int, u64p, f32p, u32p]
+    lib.vfsx_log_probs_device.argtypes = [vp, vp, C.c_uint32, C.c_int, C.c_double, C.c_int, vp, vp, C.c_uint32, C.c_uint32,
+                                          vp, vp, vp, vp, vp]
+    lib.vfsx_log_probs.argtypes = [vp, vp, C.c_uint32, C.c_int, C.c_double, C.c_int, vp, vp, C.c_uint32, C.c_uint32, vp, vp, vp, vp]
+    lib.vfsx_reserve_log_probs.argtypes = [vp, C.c_uint32, C.c_int]
+    lib.vfsx_corpus_enable_f8.argtypes = [vp, C.c_int]
+    lib.vfsx_corpus_get_rows_f8.argtypes = [vp, u64p, C.c_uint64, f32p]
+    lib.vfsx_scores_f8_device.argtypes = [vp, vp, C.c_uint32, C.c_int, C.c_int, vp, C.c_uint64, vp]
+    lib.vfsx_scores_f8.argtypes = [vp, vp, C.c_uint32, C.c_int, C.c_int, vp, C.c_uint64]
+    lib.vfsx_reserve_scores_f8.argtypes = [vp, C.c_uint32]
     for name in SYMBOLS:
         getattr(lib, name)  # AttributeError if the library does not export it
     _lib = lib

@@ -20,6 +20,7 @@
 #include <unistd.h>
 
 #include "vfsx_internal.h"
+#include "vfsx_prob.h"
 
 namespace {
 
@@ -254,6 +255,40 @@ struct VmArray {
     }
 };
 
+// One block of device memory that a call carves its workspaces from.  Once a captured graph has been given the block it is never
+// freed before its owner is: a larger call then gets another block and the old one is kept aside.
+struct WorkBlock {
+    char *p = nullptr;
+    size_t n = 0;
+    bool captured = false;
+    std::vector<void *> kept;
+    void reserve(size_t want)
+    {
+        if (want <= n)
+            return;
+        char *fresh = nullptr;
+        want = (want + (2u << 20) - 1) / (2u << 20) * (2u << 20);
+        HIP_CHECK(hipMalloc((void **)&fresh, want));
+        if (p && captured)
+            kept.push_back(p);
+        else if (p)
+            (void)hipFree(p); // (waits for the work that uses it)
+        p = fresh;
+        n = want;
+        captured = false;
+    }
+    void release()
+    {
+        for (void *k : kept)
+            (void)hipFree(k);
+        kept.clear();
+        if (p)
+            (void)hipFree(p);
+        p = nullptr;
+        n = 0;
+    }
+};
+
 } // namespace
 
 struct vfsx_corpus {
@@ -360,6 +395,13 @@ struct vfsx_corpus {
     uint32_t mirror_win_queries = 0, mirror_win_flagged = 0; // auto mirror choice: queries / margin failures seen
     uint32_t small_win_queries = 0, small_win_flagged = 0;   // calls of < 4 queries through the path: the same
     uint32_t small_off = 0;                                  // ... and how many such queries still skip it
+
+    // probabilities over the store and the 8-bit floating point copy (vfsx_prob.hip, vfsx_f8.hip)
+    VmArray va_row_inv, va_f8, va_f8_exp; // per row: 1 / |x|; e4m3 chunks; scales
+    float *d_max_norm = nullptr;          // largest finite |x| of the first prob_rows rows
+    uint64_t prob_rows = 0, f8_rows = 0;  // rows that the arrays cover
+    bool f8_enabled = false;
+    WorkBlock prob_work, prob_io;
 
     // profiling
     bool profiling = false;
@@ -1448,6 +1490,13 @@ void vfsx_corpus_destroy(vfsx_corpus *c)
     c->h_call = c->d_call = nullptr;
     c->row_idx.release();
     c->row_out.release();
+    c->prob_work.release();
+    c->prob_io.release();
+    c->va_row_inv.release();
+    c->va_f8.release();
+    c->va_f8_exp.release();
+    if (c->d_max_norm)
+        (void)hipFree(c->d_max_norm);
     c->va_corpus.release();
     c->va_norms.release();
     c->va_ids.release();
@@ -1559,7 +1608,8 @@ int vfsx_corpus_storage_info(vfsx_corpus *c, uint64_t *capacity_rows, uint64_t *
 {
     return guarded([&] {
         ready(c);
-        const VmArray *all[] = {&c->va_corpus, &c->va_norms, &c->va_ids, &c->va_mirror, &c->va_rn2, &c->va_inv};
+        const VmArray *all[] = {&c->va_corpus, &c->va_norms, &c->va_ids, &c->va_mirror, &c->va_rn2, &c->va_inv,
+                                &c->va_row_inv, &c->va_f8, &c->va_f8_exp};
         uint64_t copied = 0, bytes = 0;
         for (const VmArray *a : all) {
             copied += a->copy_bytes;
@@ -1858,6 +1908,498 @@ int vfsx_corpus_get_metadata_json(vfsx_corpus *c, uint64_t row, char *buf, uint6
             std::memcpy(buf, s.data(), n);
             buf[n] = 0;
         }
+    });
+}
+
+} // extern "C"
+
+// ---- probabilities over the store, 8-bit floating point copy (vfsx_prob.hip, vfsx_f8.hip) ----------------------------------------
+
+namespace {
+
+// the corpus' device for the time of a call, the caller's afterwards
+struct OnDevice {
+    int prev = -1;
+    explicit OnDevice(const vfsx_corpus *c)
+    {
+        if (hipGetDevice(&prev) != hipSuccess) {
+            (void)hipGetLastError();
+            prev = -1;
+        }
+        use_device(c);
+    }
+    ~OnDevice()
+    {
+        if (prev >= 0)
+            (void)hipSetDevice(prev);
+    }
+};
+
+bool is_capturing(hipStream_t s)
+{
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    HIP_CHECK(hipStreamIsCapturing(s, &st));
+    return st != hipStreamCaptureStatusNone;
+}
+
+constexpr uint64_t kProbRowPad = 256; // the per-row arrays cover whole tiles of 256 rows
+
+uint64_t prob_pad(uint64_t rows) { return (rows + kProbRowPad - 1u) / kProbRowPad * kProbRowPad; }
+
+void check_prob_rows(const vfsx_corpus *c)
+{
+    if (c->n_rows > vfsx::kMfmaMaxRows)
+        fail(VFSX_ERR_INVALID_VECTOR, "probabilities and 8-bit scores are for shards of up to " + std::to_string(vfsx::kMfmaMaxRows) + " rows");
+    if (c->dtype == VFSX_I8 && !(std::isfinite(c->scale) && c->scale != 0.0f))
+        fail(VFSX_ERR_INVALID_VECTOR, "probabilities need a finite scale factor that is not zero");
+}
+
+void fill_prob_store(vfsx_corpus *c, int source, vfsx::ProbStore &st)
+{
+    st.source = source == VFSX_SOURCE_F8 ? vfsx::kProbF8 : (c->dtype == VFSX_I8 ? vfsx::kProbI8 : vfsx::kProbF32);
+    st.rows = c->d_corpus;
+    st.f8 = (const uint4 *)c->va_f8.base;
+    st.f8_exp = (const uint32_t *)c->va_f8_exp.base;
+    st.row_inv = (const float *)c->va_row_inv.base;
+    st.max_norm = c->d_max_norm;
+    st.n_rows = (uint32_t)c->n_rows;
+    st.n_pieces = (uint32_t)((c->n_rows + vfsx::kPieceRows - 1u) / vfsx::kPieceRows);
+    st.dim = c->dim;
+    st.d_chunks = c->d_chunks;
+    st.f8_chunks = vfsx::f8_chunks(c->dim);
+    st.f8_words = vfsx::f8_exp_words(c->dim);
+}
+
+// Row norms (and the 8-bit copy) for the rows added since.  Enqueued on `s`; nothing to do in the usual call.
+void ensure_prob_rows(vfsx_corpus *c, bool f8, bool capturing, hipStream_t s)
+{
+    const bool rows_stale = c->prob_rows != c->n_rows || !c->d_max_norm, f8_stale = f8 && c->f8_rows != c->n_rows;
+    if (!rows_stale && !f8_stale)
+        return;
+    if (capturing)
+        fail(VFSX_ERR_MEMTABLE, "under graph capture: rows were added since vfsx_reserve_log_probs / vfsx_reserve_scores_f8; call it again first");
+    const uint64_t max_pad = prob_pad(c->max_rows);
+    const uint64_t pad = prob_pad(std::max<uint64_t>(c->n_rows, 1));
+    if (rows_stale) {
+        if (!c->va_row_inv.base && c->va_corpus.reserved)
+            c->va_row_inv.init(c->device, max_pad * sizeof(float));
+        c->va_row_inv.grow(pad * sizeof(float), c->prob_rows * sizeof(float), s);
+        if (!c->d_max_norm) {
+            HIP_CHECK(hipMalloc((void **)&c->d_max_norm, sizeof(float)));
+            HIP_CHECK(hipMemsetAsync(c->d_max_norm, 0, sizeof(float), s));
+        }
+        vfsx::ProbStore st{};
+        fill_prob_store(c, VFSX_SOURCE_ROWS, st);
+        HIP_CHECK(vfsx::launch_prob_rows(st, (uint32_t)c->prob_rows, (float *)c->va_row_inv.base, c->d_max_norm, s));
+        c->prob_rows = c->n_rows;
+    }
+    if (f8_stale) {
+        const size_t chunk_row = (size_t)vfsx::f8_chunks(c->dim) * 16u, exp_row = (size_t)vfsx::f8_exp_words(c->dim) * 4u;
+        if (!c->va_f8.base && c->va_corpus.reserved) {
+            c->va_f8.min_slab = 64u << 20;
+            c->va_f8.init(c->device, max_pad * chunk_row);
+            c->va_f8_exp.init(c->device, max_pad * exp_row);
+        }
+        c->va_f8.grow(pad * chunk_row, prob_pad(c->f8_rows) * chunk_row, s);
+        c->va_f8_exp.grow(pad * exp_row, prob_pad(c->f8_rows) * exp_row, s);
+        HIP_CHECK(vfsx::launch_f8_rows(c->d_corpus, c->d_chunks, c->dim, (uint32_t)c->f8_rows, (uint32_t)c->n_rows, (uint32_t)pad,
+                                       (uint4 *)c->va_f8.base, (uint32_t *)c->va_f8_exp.base, s));
+        c->f8_rows = c->n_rows;
+    }
+}
+
+void free_f8(vfsx_corpus *c)
+{
+    c->va_f8.release();
+    c->va_f8_exp.release();
+    c->f8_rows = 0;
+}
+
+// workspaces of one round of queries, carved from c->prob_work
+struct ProbCarve {
+    uint32_t round = 0, pad = 0; // queries per round; rounded up to whole tiles
+    size_t fac, eps, norm, q8, q8_exp, pieces, groups, bytes;
+};
+constexpr uint32_t kProbQueryTile = 256;
+constexpr size_t kProbRoundBytes = 512u << 20; // statistics of one round of queries
+
+ProbCarve prob_carve(const vfsx_corpus *c, uint32_t nq, bool f8, bool statistics)
+{
+    ProbCarve w{};
+    const uint64_t n_pieces = (c->n_rows + vfsx::kPieceRows - 1u) / vfsx::kPieceRows;
+    const uint64_t per_q = n_pieces * (sizeof(float4) + vfsx::kGroupsPerPiece * sizeof(float));
+    uint64_t round = 32768;
+    if (statistics && per_q)
+        round = std::min<uint64_t>(round, std::max<uint64_t>(kProbQueryTile, kProbRoundBytes / per_q / kProbQueryTile * kProbQueryTile));
+    w.round = (uint32_t)std::min<uint64_t>(round, nq);
+    w.pad = (w.round + kProbQueryTile - 1u) / kProbQueryTile * kProbQueryTile;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255u) / 256u * 256u;
+        return here;
+    };
+    w.norm = take(w.pad * sizeof(double));
+    w.fac = take(w.pad * sizeof(float));
+    w.eps = take(w.pad * sizeof(float));
+    w.q8 = take(f8 ? (size_t)w.pad * vfsx::f8_chunks(c->dim) * 16u : 0);
+    w.q8_exp = take(f8 ? (size_t)w.pad * vfsx::f8_exp_words(c->dim) * 4u : 0);
+    w.pieces = take(statistics ? (size_t)w.round * n_pieces * sizeof(float4) : 0);
+    w.groups = take(statistics ? (size_t)w.round * n_pieces * vfsx::kGroupsPerPiece * sizeof(float) : 0);
+    w.bytes = at;
+    return w;
+}
+
+void reserve_prob_work(vfsx_corpus *c, const ProbCarve &w, bool capturing)
+{
+    if (capturing) {
+        if (w.bytes > c->prob_work.n)
+            fail(VFSX_ERR_MEMTABLE, "under graph capture: call vfsx_reserve_log_probs / vfsx_reserve_scores_f8 with these sizes first");
+        c->prob_work.captured = true;
+        return;
+    }
+    c->prob_work.reserve(w.bytes);
+}
+
+void prepare_queries(const vfsx::ProbStore &st, const ProbCarve &w, char *base, const float *d_queries, uint32_t nq, bool f8,
+                     vfsx::ProbQueries &qs, hipStream_t s)
+{
+    qs.q = d_queries;
+    qs.fac = (const float *)(base + w.fac);
+    qs.eps = (const float *)(base + w.eps);
+    qs.norm = (const double *)(base + w.norm);
+    qs.q8 = (const uint4 *)(base + w.q8);
+    qs.q8_exp = (const uint32_t *)(base + w.q8_exp);
+    qs.nq = nq;
+    HIP_CHECK(vfsx::launch_prob_queries(st, d_queries, nq, (float *)(base + w.fac), (float *)(base + w.eps), (double *)(base + w.norm), s));
+    if (f8)
+        HIP_CHECK(vfsx::launch_f8_queries(d_queries, nq, st.dim, (nq + kProbQueryTile - 1u) / kProbQueryTile * kProbQueryTile,
+                                          (uint4 *)(base + w.q8), (uint32_t *)(base + w.q8_exp), s));
+}
+
+void check_similarity(int similarity)
+{
+    if (similarity != VFSX_SIM_DOT && similarity != VFSX_SIM_COSINE)
+        fail(VFSX_ERR_INVALID_VECTOR, "unknown similarity");
+}
+
+void check_source(const vfsx_corpus *c, int source)
+{
+    if (source != VFSX_SOURCE_ROWS && source != VFSX_SOURCE_F8)
+        fail(VFSX_ERR_INVALID_VECTOR, "unknown source of the rows");
+    if (source == VFSX_SOURCE_F8 && !c->f8_enabled)
+        fail(VFSX_ERR_INVALID_VECTOR, "the 8-bit floating point copy is off: call vfsx_corpus_enable_f8 first");
+}
+
+struct LogProbsArgs {
+    const float *queries;
+    uint32_t nq;
+    int similarity;
+    double temperature;
+    int source;
+    const float *bias;
+    const uint64_t *rows;
+    uint32_t n_given, k;
+    float *log_probs, *lse, *entropy;
+    vfsx_hit *top;
+};
+
+void check_log_probs(const vfsx_corpus *c, const LogProbsArgs &a)
+{
+    check_similarity(a.similarity);
+    check_source(c, a.source);
+    check_prob_rows(c);
+    if (!(a.temperature > 0.0) || !std::isfinite(a.temperature) || !std::isfinite((float)(1.0 / a.temperature)) || (float)(1.0 / a.temperature) == 0.0f)
+        fail(VFSX_ERR_INVALID_VECTOR, "temperature must be a positive number whose inverse is one in f32");
+    if (a.k > VFSX_LOG_PROBS_MAX_K)
+        fail(VFSX_ERR_INVALID_VECTOR, "k (top rows) must be in 0.." + std::to_string(VFSX_LOG_PROBS_MAX_K));
+    if (a.nq == 0)
+        return;
+    if (!a.queries)
+        fail(VFSX_ERR_INVALID_VECTOR, "null query buffer");
+    if (a.n_given && (!a.rows || !a.log_probs))
+        fail(VFSX_ERR_INVALID_VECTOR, "null buffer of the given rows");
+    if (a.k && !a.top)
+        fail(VFSX_ERR_INVALID_VECTOR, "null buffer of the top rows");
+    if (!a.n_given && !a.k && !a.lse && !a.entropy)
+        fail(VFSX_ERR_INVALID_VECTOR, "no output buffer");
+}
+
+// device buffers, checked; the corpus' device is current
+void log_probs_impl(vfsx_corpus *c, const LogProbsArgs &a, hipStream_t s, bool capturing)
+{
+    if (a.nq == 0)
+        return;
+    if (!capturing)
+        chain_search_stream(c, s);
+    const bool f8 = a.source == VFSX_SOURCE_F8;
+    ensure_prob_rows(c, f8, capturing, s);
+    const ProbCarve w = prob_carve(c, a.nq, f8, true);
+    reserve_prob_work(c, w, capturing);
+    char *base = c->prob_work.p;
+    vfsx::ProbStore st{};
+    fill_prob_store(c, a.source, st);
+    st.cosine = a.similarity == VFSX_SIM_COSINE;
+    st.bias = a.bias;
+    const double scale = st.source == vfsx::kProbI8 ? (double)c->scale : 1.0;
+    st.divide = a.temperature * (st.cosine ? (scale < 0 ? -1.0 : 1.0) : scale);
+    for (uint32_t q0 = 0; q0 < a.nq; q0 += w.round) {
+        const uint32_t qn = std::min(w.round, a.nq - q0);
+        vfsx::ProbQueries qs{};
+        prepare_queries(st, w, base, a.queries + (size_t)q0 * c->dim, qn, f8, qs, s);
+        float4 *pieces = (float4 *)(base + w.pieces);
+        float *groups = (float *)(base + w.groups);
+        HIP_CHECK(vfsx::launch_prob_pieces(st, qs, pieces, groups, s));
+        vfsx::ProbFinish f{};
+        f.pieces = pieces;
+        f.groups = groups;
+        f.given = a.n_given ? a.rows + (size_t)q0 * a.n_given : nullptr;
+        f.log_probs = a.n_given ? a.log_probs + (size_t)q0 * a.n_given : nullptr;
+        f.n_given = a.n_given;
+        f.lse = a.lse ? a.lse + q0 : nullptr;
+        f.entropy = a.entropy ? a.entropy + q0 : nullptr;
+        f.top = a.k ? a.top + (size_t)q0 * a.k : nullptr;
+        f.k = a.k;
+        f.ids = c->explicit_ids ? c->d_ids : nullptr;
+        f.row_base = c->row_base;
+        f.id_base = c->id_base;
+        HIP_CHECK(vfsx::launch_prob_finish(st, qs, f, s));
+    }
+}
+
+void scores_f8_impl(vfsx_corpus *c, const float *d_queries, uint32_t nq, int similarity, int out_dtype, void *d_out, uint64_t ld,
+                    hipStream_t s, bool capturing)
+{
+    if (nq == 0 || c->n_rows == 0)
+        return;
+    if (!capturing)
+        chain_search_stream(c, s);
+    ensure_prob_rows(c, true, capturing, s);
+    const ProbCarve w = prob_carve(c, nq, true, false);
+    reserve_prob_work(c, w, capturing);
+    vfsx::ProbStore st{};
+    fill_prob_store(c, VFSX_SOURCE_F8, st);
+    st.cosine = similarity == VFSX_SIM_COSINE;
+    st.divide = 1.0;
+    const size_t elem = out_dtype == VFSX_SCORES_BF16 ? 2 : 4;
+    for (uint32_t q0 = 0; q0 < nq; q0 += w.round) {
+        const uint32_t qn = std::min(w.round, nq - q0);
+        vfsx::ProbQueries qs{};
+        prepare_queries(st, w, c->prob_work.p, d_queries + (size_t)q0 * c->dim, qn, true, qs, s);
+        HIP_CHECK(vfsx::launch_f8_scores(st, qs, (char *)d_out + (size_t)q0 * ld * elem, ld, out_dtype == VFSX_SCORES_BF16, s));
+    }
+}
+
+void check_scores(const vfsx_corpus *c, const float *queries, uint32_t nq, int similarity, int out_dtype, const void *out, uint64_t &ld)
+{
+    check_similarity(similarity);
+    check_source(c, VFSX_SOURCE_F8);
+    check_prob_rows(c);
+    if (out_dtype != VFSX_SCORES_F32 && out_dtype != VFSX_SCORES_BF16)
+        fail(VFSX_ERR_INVALID_VECTOR, "unknown type of the scores");
+    if (ld == 0)
+        ld = c->n_rows;
+    if (ld < c->n_rows)
+        fail(VFSX_ERR_INVALID_VECTOR, "ld must be at least the number of rows");
+    if (nq && c->n_rows && (!queries || !out))
+        fail(VFSX_ERR_INVALID_VECTOR, "null query/output buffer");
+}
+
+// `ready` for calls that may be captured: committing staged rows copies and maps memory, which a capture does not allow
+vfsx_corpus *ready_on(vfsx_corpus *c, hipStream_t s, bool &capturing)
+{
+    checked(c);
+    capturing = is_capturing(s);
+    if (capturing && c->pend_n)
+        fail(VFSX_ERR_MEMTABLE, "under graph capture: appended rows wait in the insert batch; call vfsx_corpus_commit first");
+    commit_pending(c);
+    return c;
+}
+
+} // namespace
+
+extern "C" {
+
+int vfsx_log_probs_device(vfsx_corpus *c, const float *d_queries, uint32_t nq, int similarity, double temperature, int source,
+                          const float *d_bias, const uint64_t *d_rows, uint32_t n_given, uint32_t k, float *d_log_probs,
+                          float *d_lse, float *d_entropy, vfsx_hit *d_top, void *stream)
+{
+    return guarded([&] {
+        checked(c);
+        OnDevice on(c);
+        bool capturing = false;
+        ready_on(c, (hipStream_t)stream, capturing);
+        const LogProbsArgs a{d_queries, nq, similarity, temperature, source, d_bias, d_rows, n_given, k, d_log_probs, d_lse, d_entropy, d_top};
+        check_log_probs(c, a);
+        log_probs_impl(c, a, (hipStream_t)stream, capturing);
+    });
+}
+
+int vfsx_log_probs(vfsx_corpus *c, const float *queries, uint32_t nq, int similarity, double temperature, int source,
+                   const float *bias, const uint64_t *rows, uint32_t n_given, uint32_t k, float *log_probs, float *lse,
+                   float *entropy, vfsx_hit *top)
+{
+    return guarded([&] {
+        checked(c);
+        OnDevice on(c);
+        ready(c);
+        LogProbsArgs a{queries, nq, similarity, temperature, source, bias, rows, n_given, k, log_probs, lse, entropy, top};
+        check_log_probs(c, a);
+        if (nq == 0)
+            return;
+        hipStream_t s = c->stream;
+        size_t at = 0;
+        auto take = [&](size_t bytes) {
+            const size_t here = at;
+            at += (bytes + 255u) / 256u * 256u;
+            return here;
+        };
+        const size_t q_b = (size_t)nq * c->dim * 4u, bias_b = bias ? (size_t)c->n_rows * 4u : 0, given = (size_t)nq * n_given;
+        const size_t top_b = (size_t)nq * k * sizeof(vfsx_hit);
+        const size_t o_q = take(q_b), o_bias = take(bias_b), o_rows = take(given * 8u), o_lp = take(given * 4u), o_lse = take(nq * 4u),
+                     o_ent = take(nq * 4u), o_top = take(top_b);
+        c->prob_io.reserve(at);
+        char *base = c->prob_io.p;
+        HIP_CHECK(hipMemcpyAsync(base + o_q, queries, q_b, hipMemcpyHostToDevice, s));
+        if (bias_b)
+            HIP_CHECK(hipMemcpyAsync(base + o_bias, bias, bias_b, hipMemcpyHostToDevice, s));
+        if (given)
+            HIP_CHECK(hipMemcpyAsync(base + o_rows, rows, given * 8u, hipMemcpyHostToDevice, s));
+        a.queries = (const float *)(base + o_q);
+        a.bias = bias ? (const float *)(base + o_bias) : nullptr;
+        a.rows = (const uint64_t *)(base + o_rows);
+        a.log_probs = (float *)(base + o_lp);
+        a.lse = (float *)(base + o_lse);
+        a.entropy = (float *)(base + o_ent);
+        a.top = (vfsx_hit *)(base + o_top);
+        log_probs_impl(c, a, s, false);
+        if (given)
+            HIP_CHECK(hipMemcpyAsync(log_probs, base + o_lp, given * 4u, hipMemcpyDeviceToHost, s));
+        if (lse)
+            HIP_CHECK(hipMemcpyAsync(lse, base + o_lse, nq * 4u, hipMemcpyDeviceToHost, s));
+        if (entropy)
+            HIP_CHECK(hipMemcpyAsync(entropy, base + o_ent, nq * 4u, hipMemcpyDeviceToHost, s));
+        if (k)
+            HIP_CHECK(hipMemcpyAsync(top, base + o_top, top_b, hipMemcpyDeviceToHost, s));
+        HIP_CHECK(hipStreamSynchronize(s));
+    });
+}
+
+int vfsx_reserve_log_probs(vfsx_corpus *c, uint32_t nq, int source)
+{
+    return guarded([&] {
+        checked(c);
+        OnDevice on(c);
+        ready(c);
+        check_source(c, source);
+        check_prob_rows(c);
+        chain_search_stream(c, c->stream);
+        ensure_prob_rows(c, source == VFSX_SOURCE_F8, false, c->stream);
+        c->prob_work.reserve(prob_carve(c, nq, source == VFSX_SOURCE_F8, true).bytes);
+        HIP_CHECK(hipStreamSynchronize(c->stream));
+    });
+}
+
+int vfsx_corpus_enable_f8(vfsx_corpus *c, int enable)
+{
+    return guarded([&] {
+        checked(c);
+        OnDevice on(c);
+        ready(c);
+        if (c->dtype != VFSX_F32)
+            fail(VFSX_ERR_INVALID_VECTOR, "the 8-bit floating point copy is for VFSX_F32 corpora");
+        if (!enable) {
+            if (c->f8_enabled)
+                HIP_CHECK(hipDeviceSynchronize()); // calls that read the copy may still run
+            c->f8_enabled = false;
+            free_f8(c);
+            return;
+        }
+        check_prob_rows(c);
+        chain_search_stream(c, c->stream);
+        ensure_prob_rows(c, true, false, c->stream);
+        HIP_CHECK(hipStreamSynchronize(c->stream));
+        c->f8_enabled = true;
+    });
+}
+
+int vfsx_corpus_get_rows_f8(vfsx_corpus *c, const uint64_t *rows, uint64_t n, float *out)
+{
+    return guarded([&] {
+        checked(c);
+        OnDevice on(c);
+        ready(c);
+        check_source(c, VFSX_SOURCE_F8);
+        if (n == 0)
+            return;
+        if (!rows || !out)
+            fail(VFSX_ERR_INVALID_VECTOR, "null buffer");
+        for (uint64_t i = 0; i < n; ++i)
+            if (rows[i] >= c->n_rows)
+                fail(VFSX_ERR_INVALID_VECTOR, "row index out of range");
+        hipStream_t s = c->stream;
+        chain_search_stream(c, s);
+        ensure_prob_rows(c, true, false, s);
+        c->row_idx.reserve(n);
+        c->row_out.reserve((size_t)n * c->dim * 4u);
+        HIP_CHECK(hipMemcpyAsync(c->row_idx.p, rows, n * sizeof(uint64_t), hipMemcpyHostToDevice, s));
+        HIP_CHECK(vfsx::launch_f8_get_rows((const uint4 *)c->va_f8.base, (const uint32_t *)c->va_f8_exp.base, c->dim, c->row_idx.p, n,
+                                           (float *)c->row_out.p, s));
+        HIP_CHECK(hipMemcpyAsync(out, c->row_out.p, (size_t)n * c->dim * 4u, hipMemcpyDeviceToHost, s));
+        HIP_CHECK(hipStreamSynchronize(s));
+    });
+}
+
+int vfsx_scores_f8_device(vfsx_corpus *c, const float *d_queries, uint32_t nq, int similarity, int out_dtype, void *d_out, uint64_t ld,
+                          void *stream)
+{
+    return guarded([&] {
+        checked(c);
+        OnDevice on(c);
+        bool capturing = false;
+        ready_on(c, (hipStream_t)stream, capturing);
+        check_scores(c, d_queries, nq, similarity, out_dtype, d_out, ld);
+        scores_f8_impl(c, d_queries, nq, similarity, out_dtype, d_out, ld, (hipStream_t)stream, capturing);
+    });
+}
+
+int vfsx_scores_f8(vfsx_corpus *c, const float *queries, uint32_t nq, int similarity, int out_dtype, void *out, uint64_t ld)
+{
+    return guarded([&] {
+        checked(c);
+        OnDevice on(c);
+        ready(c);
+        check_scores(c, queries, nq, similarity, out_dtype, out, ld);
+        if (nq == 0 || c->n_rows == 0)
+            return;
+        hipStream_t s = c->stream;
+        const size_t elem = out_dtype == VFSX_SCORES_BF16 ? 2 : 4, row = (size_t)c->n_rows * elem;
+        const uint32_t round = (uint32_t)std::min<uint64_t>(nq, std::max<uint64_t>(1, (256ull << 20) / row)); // 256 MiB of scores at a time
+        const size_t q_b = ((size_t)round * c->dim * 4u + 255u) / 256u * 256u;
+        c->prob_io.reserve(q_b + round * row);
+        for (uint32_t q0 = 0; q0 < nq; q0 += round) {
+            const uint32_t qn = std::min(round, nq - q0);
+            HIP_CHECK(hipMemcpyAsync(c->prob_io.p, queries + (size_t)q0 * c->dim, (size_t)qn * c->dim * 4u, hipMemcpyHostToDevice, s));
+            scores_f8_impl(c, (const float *)c->prob_io.p, qn, similarity, out_dtype, c->prob_io.p + q_b, c->n_rows, s, false);
+            for (uint32_t q = 0; q < qn; ++q)
+                HIP_CHECK(hipMemcpyAsync((char *)out + (size_t)(q0 + q) * ld * elem, c->prob_io.p + q_b + q * row, row, hipMemcpyDeviceToHost, s));
+            HIP_CHECK(hipStreamSynchronize(s));
+        }
+    });
+}
+
+int vfsx_reserve_scores_f8(vfsx_corpus *c, uint32_t nq)
+{
+    return guarded([&] {
+        checked(c);
+        OnDevice on(c);
+        ready(c);
+        check_source(c, VFSX_SOURCE_F8);
+        check_prob_rows(c);
+        chain_search_stream(c, c->stream);
+        ensure_prob_rows(c, true, false, c->stream);
+        c->prob_work.reserve(prob_carve(c, nq, true, false).bytes);
+        HIP_CHECK(hipStreamSynchronize(c->stream));
     });
 }
 

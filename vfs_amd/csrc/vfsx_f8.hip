@@ -1,0 +1,188 @@
+// vfsx_f8.hip -- the 8-bit floating point copy of a store and its product with a batch of queries.
+//
+//   block kb of a row = its elements 128 kb .. 128 kb + 127 (zeros beyond dim)
+//   e  = the least integer >= -127 with max|x| <= 448 * 2^e  (0 for a block of zeros),  x8 = e4m3(x * 2^-e), to nearest even
+//   s(q, x) = sum_kb 2^(e_q,kb + e_x,kb) * sum_t q8_t x8_t
+//
+// The scale is a power of two on purpose: scaling a row by it rounds nothing (so the copy's only error is e4m3's own
+// half step, 2^-4 of the value), and it is what v_mfma_scale_f32_32x32x64_f8f6f4 applies to its operands by itself -- a scale with a
+// mantissa would cost two VALU operations for each product of a block, about as long as the matrix instruction takes.
+// A block that holds a NaN or an infinity becomes all NaN (e = 0).
+#include <hip/hip_runtime.h>
+
+#include "vfsx_internal.h"
+#include "vfsx_prob.h"
+#include "vfsx_prob_device.h"
+
+namespace vfsx {
+
+namespace {
+
+// e of a block from the bits of max|x|: 448 = 1.75 * 2^8, so e = (exponent of max) - 8, one more when its leading digits pass 1.75
+__device__ __forceinline__ int f8_exponent(float top)
+{
+    const uint32_t b = __float_as_uint(top);
+    if (b == 0u || b >= 0x7f800000u)
+        return 0;
+    const int e = (int)(b >> 23) - 135 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < -127 ? -127 : e;
+}
+
+// four values -> four e4m3 bytes; `by` = 2^-e (never subnormal: e <= 120)
+__device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d, float by)
+{
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * by, b * by, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * by, d * by, w, true);
+}
+
+__device__ __forceinline__ float pow2_neg(int e) { return __uint_as_float((uint32_t)(127 - e) << 23); }
+
+// One lane per row, one wave per (row-block, dword of four scales): reads the row's f32 chunks twice (maximum, then the values;
+// the second read comes from the cache), writes 16-byte chunks back to back over the 64 lanes.  Bound by reading the store
+// once; runs when rows were added.
+__global__ __launch_bounds__(64) void f8_rows_kernel(const uint4 *__restrict__ rows, uint32_t d_chunks, uint32_t dim, uint32_t row0,
+                                                     uint32_t n_rows, uint32_t chunks8, uint32_t words, uint4 *__restrict__ f8,
+                                                     uint32_t *__restrict__ f8_exp)
+{
+    const uint32_t lane = threadIdx.x, rb = row0 / 64u + blockIdx.x, word = blockIdx.y;
+    const uint64_t row = (uint64_t)rb * 64u + lane;
+    if (row < row0)
+        return; // (an append adds rows from row0 on; the others of this row-block are there)
+    const uint4 *src = rows + (size_t)rb * d_chunks * 64u + lane;
+    uint4 *dst = f8 + (size_t)rb * chunks8 * 64u + lane;
+    uint32_t exps = 0;
+    for (uint32_t j = 0; j < 4u; ++j) {
+        const uint32_t kb = word * 4u + j;
+        int e = 0;
+        float top = 0.0f, by = 1.0f;
+        bool bad = false;
+        const uint32_t c0 = kb * 32u, c1 = min(c0 + 32u, d_chunks); // f32 chunks of this block that exist
+        if (row < n_rows) {
+            for (uint32_t c = c0; c < c1; ++c) { // (a row's elements beyond dim are stored as zeros)
+                const uint4 v = src[(size_t)c * 64u];
+                const float a[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+                for (int i = 0; i < 4; ++i) {
+                    top = fmaxf(top, fabsf(a[i]));
+                    bad = bad || !(fabsf(a[i]) < __builtin_inff());
+                }
+            }
+            e = bad ? 0 : f8_exponent(top);
+            by = pow2_neg(e);
+        }
+        exps |= (uint32_t)(e + 127) << (8u * j);
+        if (kb * kF8ChunksPerBlock >= chunks8)
+            continue;
+        for (uint32_t c8 = 0; c8 < kF8ChunksPerBlock; ++c8) {
+            uint32_t w[4];
+            for (uint32_t i = 0; i < 4u; ++i) {
+                const uint32_t c = c0 + c8 * 4u + i;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row < n_rows && c < c1)
+                    v = src[(size_t)c * 64u];
+                w[i] = bad ? 0x7f7f7f7fu
+                           : f8_pack4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w), by);
+            }
+            dst[(size_t)(kb * kF8ChunksPerBlock + c8) * 64u] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    f8_exp[((size_t)rb * words + word) * 64u + lane] = exps;
+}
+
+// Queries, row-major f32 -> the same layout.  One wave per (query, dword of four scales), two elements of a block per lane; queries
+// beyond nq become zeros (the product computes whole tiles of queries).
+__global__ __launch_bounds__(64) void f8_queries_kernel(const float *__restrict__ q, uint32_t nq, uint32_t dim, uint32_t chunks8,
+                                                        uint32_t words, uint4 *__restrict__ q8, uint32_t *__restrict__ q8_exp)
+{
+    const uint32_t lane = threadIdx.x, qi = blockIdx.x, word = blockIdx.y;
+    const float *src = q + (size_t)qi * dim;
+    uint8_t *dst = (uint8_t *)(q8 + (size_t)(qi / 64u) * chunks8 * 64u + (qi & 63u));
+    uint32_t exps = 0;
+    for (uint32_t j = 0; j < 4u; ++j) {
+        const uint32_t kb = word * 4u + j, k = kb * kF8Block + 2u * lane;
+        const float a = qi < nq && k < dim ? src[k] : 0.0f, b = qi < nq && k + 1u < dim ? src[k + 1u] : 0.0f;
+        float top = fmaxf(fabsf(a), fabsf(b));
+        const bool bad = __any(!(fabsf(a) < __builtin_inff()) || !(fabsf(b) < __builtin_inff()));
+        for (int o = 32; o; o >>= 1)
+            top = fmaxf(top, __shfl_xor(top, o, 64));
+        const int e = bad ? 0 : f8_exponent(top);
+        exps |= (uint32_t)(e + 127) << (8u * j);
+        if (kb * kF8ChunksPerBlock < chunks8) {
+            const float by = pow2_neg(e);
+            const uint16_t w = bad ? (uint16_t)0x7f7f : (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(a * by, b * by, 0, false);
+            // element k of a row lies in byte k % 16 of chunk k / 16
+            *(uint16_t *)(dst + (size_t)(k / 16u) * 1024u + (k & 15u)) = w;
+        }
+    }
+    if (lane == 0)
+        q8_exp[((size_t)(qi / 64u) * words + word) * 64u + (qi & 63u)] = exps;
+}
+
+__global__ void f8_get_rows_kernel(const uint4 *__restrict__ f8, const uint32_t *__restrict__ f8_exp, uint32_t dim, uint32_t chunks8,
+                                   uint32_t words, const uint64_t *__restrict__ at, uint64_t n, float *__restrict__ out)
+{
+    const uint64_t t = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (t >= n * dim)
+        return;
+    const uint64_t row = at[t / dim];
+    const uint32_t k = (uint32_t)(t % dim);
+    const uint8_t byte = ((const uint8_t *)(f8 + ((size_t)(row / 64u) * chunks8 + k / 16u) * 64u + (row & 63u)))[k & 15u];
+    const int e = f8_exp_of(f8_exp + (size_t)(row / 64u) * words * 64u + (row & 63u), k / kF8Block);
+    out[t] = ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)byte, 0), e);
+}
+
+// ---- scores, one thread per (query, row) ------------------------------------------------------------------------------------
+template <typename OUT>
+__global__ __launch_bounds__(256) void f8_scores_kernel(ProbStore st, ProbQueries qs, OUT *__restrict__ out, uint64_t ld)
+{
+    const uint32_t row = blockIdx.x * 256u + threadIdx.x, qi = blockIdx.y;
+    if (row >= st.n_rows)
+        return;
+    float s = f8_dot(st, qs, qi, row);
+    if (st.cosine) {
+        const float inv = st.row_inv[row];
+        s = qs.norm[qi] > 0.0 && inv >= 0.0f ? s * qs.fac[qi] * inv : __builtin_nanf("");
+    } else {
+        s *= qs.fac[qi];
+    }
+    out[(size_t)qi * ld + row] = (OUT)s;
+}
+
+} // namespace
+
+hipError_t launch_f8_rows(const uint4 *rows, uint32_t d_chunks, uint32_t dim, uint32_t row0, uint32_t n_rows, uint32_t n_pad,
+                          uint4 *f8, uint32_t *f8_exp, hipStream_t s)
+{
+    if (n_pad <= row0)
+        return hipSuccess;
+    f8_rows_kernel<<<dim3((n_pad - row0 / 64u * 64u) / 64u, f8_exp_words(dim)), 64, 0, s>>>(
+        rows, d_chunks, dim, row0, n_rows, f8_chunks(dim), f8_exp_words(dim), f8, f8_exp);
+    return hipGetLastError();
+}
+
+hipError_t launch_f8_queries(const float *q, uint32_t nq, uint32_t dim, uint32_t nq_pad, uint4 *q8, uint32_t *q8_exp, hipStream_t s)
+{
+    f8_queries_kernel<<<dim3(nq_pad, f8_exp_words(dim)), 64, 0, s>>>(q, nq, dim, f8_chunks(dim), f8_exp_words(dim), q8, q8_exp);
+    return hipGetLastError();
+}
+
+hipError_t launch_f8_get_rows(const uint4 *f8, const uint32_t *f8_exp, uint32_t dim, const uint64_t *d_rows, uint64_t n, float *out,
+                              hipStream_t s)
+{
+    const uint64_t blocks = (n * dim + 255u) / 256u;
+    if (blocks > 0x7fffffffull)
+        return hipErrorInvalidValue;
+    f8_get_rows_kernel<<<(uint32_t)blocks, 256, 0, s>>>(f8, f8_exp, dim, f8_chunks(dim), f8_exp_words(dim), d_rows, n, out);
+    return hipGetLastError();
+}
+
+hipError_t launch_f8_scores(const ProbStore &st, const ProbQueries &q, void *out, uint64_t ld, int bf16, hipStream_t s)
+{
+    const dim3 grid((st.n_rows + 255u) / 256u, q.nq);
+    if (bf16)
+        f8_scores_kernel<__bf16><<<grid, 256, 0, s>>>(st, q, (__bf16 *)out, ld);
+    else
+        f8_scores_kernel<float><<<grid, 256, 0, s>>>(st, q, (float *)out, ld);
+    return hipGetLastError();
+}
+
+} // namespace vfsx

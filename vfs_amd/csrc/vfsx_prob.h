@@ -1,0 +1,81 @@
+// vfsx_prob.h -- probabilities over the store and the 8-bit floating point product: what vfsx_prob.hip and vfsx_f8.hip
+// share with the C-ABI layer (vfsx_api.cpp).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "vfsx.h"
+
+namespace vfsx {
+
+// ---- 8-bit floating point copy ("f8"): e4m3 bytes in the rb64 layout, K padded with zeros to whole blocks of 128 ----------
+constexpr uint32_t kF8Block = 128;                 // elements that share one scale
+constexpr uint32_t kF8ChunksPerBlock = 8;          // 16-byte chunks of one block
+inline uint32_t f8_blocks(uint32_t dim) { return (dim + kF8Block - 1u) / kF8Block; }
+inline uint32_t f8_chunks(uint32_t dim) { return f8_blocks(dim) * kF8ChunksPerBlock; }
+// scales: e8m0 bytes (the exponent + 127) as the matrix instruction takes them, four consecutive blocks of one row in a
+// dword, [row-block][f8_exp_words][64 rows]
+inline uint32_t f8_exp_words(uint32_t dim) { return (f8_blocks(dim) + 3u) / 4u; }
+
+// ---- log probabilities: pieces and groups -----------------------------------------------------------------------------------
+// The first pass leaves, for each query, one (max, sum, weighted sum) per PIECE of 128 rows and one maximum per GROUP of
+// 16 rows; the second pass (one workgroup per query) joins them and looks into the few groups that can hold a result.
+constexpr uint32_t kPieceRows = 128;
+constexpr uint32_t kGroupRows = 16;
+constexpr uint32_t kGroupsPerPiece = kPieceRows / kGroupRows;
+
+enum ProbSource { kProbF32 = 0, kProbI8 = 1, kProbF8 = 2 };
+
+// what a pass over the store reads; the same for every query
+struct ProbStore {
+    int source;            // ProbSource
+    int cosine;
+    const uint4 *rows;     // rb64: f32 or int8
+    const uint4 *f8;       // rb64: e4m3 (source f8)
+    const uint32_t *f8_exp;
+    const float *row_inv;  // [n_rows] 1 / |x|; < 0: the row has no cosine
+    const float *max_norm; // device scalar: the largest finite |x| of the store
+    const float *bias;     // [n_rows] or nullptr
+    uint32_t n_rows, n_pieces;
+    uint32_t dim, d_chunks, f8_chunks, f8_words;
+    double divide;         // what a product is divided by before the norms: T, times the int8 scale for a dot product
+};
+
+// the queries of one launch, prepared (prob_query_kernel)
+struct ProbQueries {
+    const float *q;        // [nq][dim] as the caller gave them
+    const uint4 *q8;       // rb64 e4m3, whole row-blocks (source f8)
+    const uint32_t *q8_exp;
+    const float *fac;      // [nq] logit = product * fac [* row_inv] + bias
+    const float *eps;      // [nq] how far a first-pass logit may be from its value, relative to its row's part (see vfsx_prob.hip)
+    const double *norm;    // [nq] |q|; 0: the query has no cosine
+    uint32_t nq;
+};
+
+struct ProbFinish {
+    const float4 *pieces;  // [nq][n_pieces] (max, sum, weighted sum, 0)
+    const float *groups;   // [nq][n_pieces * kGroupsPerPiece]
+    const uint64_t *given; // [nq][n_given] global rows, or nullptr
+    const uint64_t *ids;   // explicit ids or nullptr
+    float *log_probs, *lse, *entropy;
+    vfsx_hit *top;
+    uint64_t row_base, id_base;
+    uint32_t n_given, k;
+};
+
+hipError_t launch_prob_rows(const ProbStore &st, uint32_t row0, float *row_inv, float *max_norm, hipStream_t s);
+hipError_t launch_prob_queries(const ProbStore &st, const float *q, uint32_t nq, float *fac, float *eps, double *norm, hipStream_t s);
+hipError_t launch_prob_pieces(const ProbStore &st, const ProbQueries &q, float4 *pieces, float *groups, hipStream_t s);
+hipError_t launch_prob_finish(const ProbStore &st, const ProbQueries &q, const ProbFinish &f, hipStream_t s);
+
+// vfsx_f8.hip
+hipError_t launch_f8_rows(const uint4 *rows, uint32_t d_chunks, uint32_t dim, uint32_t row0, uint32_t n_rows, uint32_t n_pad,
+                          uint4 *f8, uint32_t *f8_exp, hipStream_t s);
+hipError_t launch_f8_queries(const float *q, uint32_t nq, uint32_t dim, uint32_t nq_pad, uint4 *q8, uint32_t *q8_exp, hipStream_t s);
+hipError_t launch_f8_get_rows(const uint4 *f8, const uint32_t *f8_exp, uint32_t dim, const uint64_t *d_rows, uint64_t n, float *out,
+                              hipStream_t s);
+// out[nq][ld]: f32 (bf16 = 0) or bf16
+hipError_t launch_f8_scores(const ProbStore &st, const ProbQueries &q, void *out, uint64_t ld, int bf16, hipStream_t s);
+
+} // namespace vfsx

@@ -104,6 +104,34 @@ public:
         return b;
     }
 
+    // Softmax of sim(query, row) / temperature over the whole store (include/vfsx.h, vfsx_log_probs): log probabilities of the
+    // given rows [nq][n_given], log of the sum and entropy [nq], the k most probable rows [nq][k].
+    struct LogProbs {
+        std::vector<float> log_probs, lse, entropy;
+        std::vector<vfsx_hit> top;
+    };
+    LogProbs log_probs(const float *queries, uint32_t nq, const uint64_t *rows, uint32_t n_given, uint32_t k,
+                       vfsx_similarity similarity = VFSX_SIM_DOT, double temperature = 1.0, const float *bias = nullptr,
+                       vfsx_source source = VFSX_SOURCE_ROWS)
+    {
+        LogProbs r;
+        r.log_probs.resize((size_t)nq * n_given);
+        r.lse.resize(nq);
+        r.entropy.resize(nq);
+        r.top.resize((size_t)nq * k);
+        check(vfsx_log_probs(h_, queries, nq, similarity, temperature, source, bias, rows, n_given, k, r.log_probs.data(),
+                             r.lse.data(), r.entropy.data(), r.top.data()));
+        return r;
+    }
+    // 8-bit floating point copy of an f32 store and the scores of every row through it, [nq][rows()]
+    void enable_f8(bool on = true) { check(vfsx_corpus_enable_f8(h_, on ? 1 : 0)); }
+    std::vector<float> scores_f8(const float *queries, uint32_t nq, vfsx_similarity similarity = VFSX_SIM_DOT)
+    {
+        std::vector<float> out((size_t)nq * rows());
+        check(vfsx_scores_f8(h_, queries, nq, similarity, VFSX_SCORES_F32, out.data(), 0));
+        return out;
+    }
+
 private:
     vfsx_corpus *h_ = nullptr;
     uint32_t dim_;

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import enum
-from typing import List, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -38,6 +38,20 @@ class DistanceMethod(enum.IntEnum):  # rank.rs:67-72 (declaration order)
                 "simd_cosine": DistanceMethod.SimdCosine,
                 "simd_euclidean": DistanceMethod.SimdEuclidean,
                 "euclidean_i8_domain": DistanceMethod.EuclideanI8Domain}.get(name or "", DistanceMethod.Euclidean)
+
+
+_HIT = np.dtype([("dist", np.float32), ("flags", np.uint32), ("row", np.uint64), ("id", np.uint64)])  # vfsx_hit
+
+
+class LogProbs(NamedTuple):
+    """What Corpus.log_probs returns, each with one entry (row of entries) per query."""
+    log_probs: np.ndarray      # [nq, t] of the given rows
+    lse: np.ndarray            # [nq] log of the sum of exp(logits)
+    entropy: np.ndarray        # [nq] natural units
+    top_rows: np.ndarray       # [nq, k] the most probable rows (global scan positions) ...
+    top_ids: np.ndarray        # [nq, k]
+    top_log_probs: np.ndarray  # [nq, k]
+    top_count: np.ndarray      # [nq] ... of which this many are there
 
 
 SIMD_WIDTHS = (2, 4, 8, 16, 32, 64)  # rank.rs:303,307
@@ -215,6 +229,104 @@ class Corpus:
         exact scan on the library's static device workspace; no hipMalloc / hipFree on this call."""
         _lib.check(self._lib.vfsx_search_device_noalloc(self._h, C.c_void_p(d_queries_ptr), nq, k, int(metric),
                                                         C.c_void_p(d_hits_ptr), C.c_void_p(stream_ptr)))
+
+    # -- probabilities over the store ------------------------------------------------
+    def _queries_arg(self, queries) -> np.ndarray:
+        q = np.ascontiguousarray(queries, dtype=np.float32)
+        if q.ndim == 1:
+            q = q[None, :]
+        if q.ndim != 2 or q.shape[1] != self.dim:
+            got = q.shape[1] if q.ndim == 2 else q.shape
+            raise _lib.VfsxError(_lib.ERR_INVALID_VECTOR, f"Query vector dimension mismatch. Expected {self.dim}, got {got}")
+        return q
+
+    @staticmethod
+    def _choice(table: dict, value: str, what: str) -> int:
+        try:
+            return table[value]
+        except (KeyError, TypeError):
+            raise _lib.VfsxError(_lib.ERR_INVALID_VECTOR, f"{what} must be one of {', '.join(table)}: got {value!r}") from None
+
+    def log_probs(self, queries, rows=None, k: int = 0, *, similarity: str = "dot", temperature: float = 1.0, bias=None,
+                  source: str = "rows") -> LogProbs:
+        """Softmax of sim(query, row) / temperature + bias over the whole store, for each query (vfsx_log_probs): log
+        probabilities of the given `rows` ([nq, t] or, shared by all queries, [t] global scan positions; -1 = an unused place),
+        log of the sum, entropy, and the `k` <= 128 most probable rows.  `bias` [len(self)]: -inf takes a row out.
+        source "f8" reads the 8-bit floating point copy (enable_f8)."""
+        q = self._queries_arg(queries)
+        nq = q.shape[0]
+        given = np.zeros((nq, 0), np.uint64)
+        if rows is not None:
+            given = np.asarray(rows)
+            if given.dtype.kind not in "iu":
+                raise _lib.VfsxError(_lib.ERR_INVALID_VECTOR, "rows must be integers")
+            if given.ndim == 1:
+                given = np.broadcast_to(given, (nq, given.shape[0]))
+            if given.ndim != 2 or given.shape[0] != nq:
+                raise _lib.VfsxError(_lib.ERR_INVALID_VECTOR, "rows must be [t], or [nq, t] for nq queries")
+            given = np.ascontiguousarray(given).astype(np.uint64)  # (-1 becomes ~0: no row)
+        b = None
+        if bias is not None:
+            b = np.ascontiguousarray(bias, dtype=np.float32)
+            if b.shape != (len(self),):
+                raise _lib.VfsxError(_lib.ERR_INVALID_VECTOR, "bias must have one entry per row")
+        k = int(k)
+        if k < 0:
+            raise _lib.VfsxError(_lib.ERR_INVALID_VECTOR, "k (top rows) must not be negative")
+        lp = np.zeros(given.shape, np.float32)
+        lse, entropy = np.zeros(nq, np.float32), np.zeros(nq, np.float32)
+        top = np.zeros((nq, k), dtype=_HIT)
+        _lib.check(self._lib.vfsx_log_probs(
+            self._h, q.ctypes.data, nq, self._choice(_lib.SIMILARITY, similarity, "similarity"), float(temperature),
+            self._choice(_lib.SOURCE, source, "source"), None if b is None else b.ctypes.data,
+            given.ctypes.data if given.shape[1] else None, given.shape[1], k, lp.ctypes.data if given.shape[1] else None,
+            lse.ctypes.data, entropy.ctypes.data, top.ctypes.data if k else None))
+        return LogProbs(lp, lse, entropy, top["row"], top["id"], top["dist"], (top["flags"] & 1).sum(axis=1))
+
+    def log_probs_device(self, d_queries: int, nq: int, *, d_rows: int = 0, given: int = 0, k: int = 0, similarity: str = "dot",
+                         temperature: float = 1.0, d_bias: int = 0, source: str = "rows", d_log_probs: int = 0, d_lse: int = 0,
+                         d_entropy: int = 0, d_top: int = 0, stream: int = 0) -> None:
+        """log_probs on device buffers (addresses), enqueued on `stream` (vfsx_log_probs_device)."""
+        _lib.check(self._lib.vfsx_log_probs_device(
+            self._h, d_queries, nq, self._choice(_lib.SIMILARITY, similarity, "similarity"), temperature,
+            self._choice(_lib.SOURCE, source, "source"), d_bias, d_rows, given, k, d_log_probs, d_lse, d_entropy, d_top, stream))
+
+    def reserve_log_probs(self, nq: int, source: str = "rows") -> None:
+        """Allocate for log_probs calls of up to `nq` queries: needed before one is captured into a graph."""
+        _lib.check(self._lib.vfsx_reserve_log_probs(self._h, int(nq), self._choice(_lib.SOURCE, source, "source")))
+
+    # -- 8-bit floating point copy -------------------------------------------------------
+    def enable_f8(self, enabled: bool = True) -> None:
+        """Keep an e4m3 copy of an f32 store with a power-of-two scale for each block of 128 elements
+        (vfsx_corpus_enable_f8): what scores_f8 and log_probs(source="f8") read."""
+        _lib.check(self._lib.vfsx_corpus_enable_f8(self._h, 1 if enabled else 0))
+
+    def get_rows_f8(self, rows: Sequence[int]) -> np.ndarray:
+        """The values the copy holds, as float32."""
+        idx = np.ascontiguousarray(rows, dtype=np.uint64)
+        out = np.empty((idx.size, self.dim), dtype=np.float32)
+        _lib.check(self._lib.vfsx_corpus_get_rows_f8(self._h, idx.ctypes.data_as(C.POINTER(C.c_uint64)), idx.size,
+                                                     out.ctypes.data_as(C.POINTER(C.c_float))))
+        return out
+
+    def scores_f8(self, queries, similarity: str = "dot") -> np.ndarray:
+        """[nq, len(self)] f32 scores of every row, both sides in 8-bit floating point (vfsx_scores_f8)."""
+        q = self._queries_arg(queries)
+        out = np.empty((q.shape[0], len(self)), dtype=np.float32)
+        _lib.check(self._lib.vfsx_scores_f8(self._h, q.ctypes.data, q.shape[0],
+                                            self._choice(_lib.SIMILARITY, similarity, "similarity"), 0, out.ctypes.data, 0))
+        return out
+
+    def scores_f8_device(self, d_queries: int, nq: int, d_out: int, *, ld: int = 0, dtype: str = "f32", similarity: str = "dot",
+                         stream: int = 0) -> None:
+        """scores_f8 on device buffers (addresses); dtype "f32" or "bf16", rows of `ld` elements (0: len(self))."""
+        _lib.check(self._lib.vfsx_scores_f8_device(
+            self._h, d_queries, nq, self._choice(_lib.SIMILARITY, similarity, "similarity"),
+            self._choice(_lib.SCORES_DTYPE, dtype, "dtype"), d_out, ld, stream))
+
+    def reserve_scores_f8(self, nq: int) -> None:
+        """Allocate for scores_f8 calls of up to `nq` queries: needed before one is captured into a graph."""
+        _lib.check(self._lib.vfsx_reserve_scores_f8(self._h, int(nq)))
 
     def enable_mfma(self, enabled: bool = True, mirror: str = "auto") -> None:
         """Let Cosine / Euclidean batches run on the matrix cores (results stay those of the exact scan).  f32 stores

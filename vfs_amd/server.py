@@ -383,19 +383,33 @@ class App:
                                                      if isinstance(req.get("distance_method"), str) else None)
         ef = req.get("ef_search")
         ef_search = ef if isinstance(ef, int) and not isinstance(ef, bool) and ef >= 0 else 6
+        # "temperature" (no counterpart in the reference): the hits' log probabilities under the softmax of cosine / temperature
+        # over the whole store, and its entropy -- how sure the answer is
+        temperature = req.get("temperature")
+        if temperature is not None:
+            if (isinstance(temperature, bool) or not isinstance(temperature, (int, float)) or not 1e-30 < temperature < 1e30):
+                return 400, err_body("temperature must be a positive number")
+            if method not in (vfs_amd.DistanceMethod.Cosine, vfs_amd.DistanceMethod.SimdCosine):
+                return 400, err_body("temperature needs a cosine distance_method")
         ranker = vfs_amd.Ranker(vfs_amd.SearchType.Exact, method, ef_search)
         t0 = time.perf_counter()
         try:  # ranker.search(&query, req.top_k /*batch*/, Some(ef_search) /*limit*/, manager): tcp.rs:403
             hits = ranker.search(req["values"], req["top_k"], ef_search, st.corpus)
+            lp = None
+            if temperature is not None:
+                lp = st.corpus.log_probs(req["values"], np.array([[st.row_of[vid] for vid, _ in hits]], dtype=np.int64),
+                                         similarity="cosine", temperature=temperature)
         except vfs_amd.VfsxError as e:
             return 500, err_body(f"Search error: {e}")
         ms = np.float32(np.float32(time.perf_counter() - t0) * np.float32(1000.0))
         results = []
-        for vid, dist in hits:
+        for i, (vid, dist) in enumerate(hits):
             v = st.vector(vid)
             vec = "null" if v is None else self._vector_value(*v)
-            results.append(jobj([("id", str(vid)), ("distance", fmt_f32_widened(dist)), ("vector", vec)]))
-        return 200, jobj([("results", "[" + ",".join(results) + "]"), ("query_time_ms", fmt_f32_widened(ms))])
+            more = [] if lp is None else [("log_prob", fmt_f32_widened(lp.log_probs[0, i]))]
+            results.append(jobj([("id", str(vid)), ("distance", fmt_f32_widened(dist)), ("vector", vec)] + more))
+        more = [] if lp is None else [("entropy", fmt_f32_widened(lp.entropy[0]))]
+        return 200, jobj([("results", "[" + ",".join(results) + "]"), ("query_time_ms", fmt_f32_widened(ms))] + more)
 
     def snapshot(self) -> Tuple[int, str]:  # tcp.rs:182-195, storage_manager.rs:367-410
         """Writes state/vfs_state.bin in the reference's bincode layout and flushes the memtable.
