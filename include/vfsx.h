@@ -454,6 +454,7 @@ int vfsx_corpus_scan_time_ms(vfsx_corpus *c, double *total_ms, uint64_t *launche
  * query whose squared norm is 0 in f32 has no cosine: that row is not there, for that query no row is.
  * When no row is there (an empty store, everything masked): lse = -inf, entropy = 0, log probabilities -inf, no top rows.
  * A logit that is NaN or infinite in f32 makes all results of its query NaN, and its top rows empty (flags = 0).
+ * For stores of up to 2^20 dimensions and 2^32 - 512 rows.
  */
 typedef enum vfsx_similarity { VFSX_SIM_DOT = 0, VFSX_SIM_COSINE = 1 } vfsx_similarity;
 typedef enum vfsx_source { VFSX_SOURCE_ROWS = 0, VFSX_SOURCE_F8 = 1 } vfsx_source;
@@ -498,7 +499,8 @@ typedef enum vfsx_scores_dtype { VFSX_SCORES_F32 = 0, VFSX_SCORES_BF16 = 1 } vfs
 /*
  * All scores: out[q][j] = q8 . x8_j (VFSX_SIM_DOT), divided by the norms of the f32 query and row (VFSX_SIM_COSINE; NaN where
  * one of them has none).  out is [nq][ld] f32 or bf16 with ld >= rows (0 = rows; elements beyond the rows are not written).
- * Accumulated in f32, rounded once.  Capture and workspaces as above (vfsx_reserve_scores_f8).
+ * f32: exact products, accumulated in f32.  bf16: by the 8-bit matrix instruction, whose sums of eight products are good to about 2^-13 of the
+ * largest of them, accumulated in f32, rounded to bf16 once.  Capture and workspaces as above (vfsx_reserve_scores_f8).
  */
 int vfsx_scores_f8_device(vfsx_corpus *c, const float *d_queries, uint32_t nq, int similarity, int out_dtype, void *d_out,
                           uint64_t ld, void *stream);

@@ -73,6 +73,12 @@ def test_scores_against_definition(size, similarity, dtype):
     if similarity == "cosine":
         by = np.linalg.norm(q.astype(np.float64), axis=1)[:, None] * np.linalg.norm(rows.astype(np.float64), axis=1)[None, :]
         want, tol = want / by, tol / by + 3 * 2.0**-24 * np.abs(want / by)
+    if dtype == "bf16":
+        # The 8-bit matrix instruction adds eight products at a time, aligned to the largest of them with a step of 2^-13 of it (beside 2^16 a
+        # product of 2^3 counts and one of 2^2 does not): each of the seven others is off by at most a step, 7 * 2^-13 < 2^-10 of the
+        # largest, which is at most 2^-10 of the sum of the magnitudes.
+        mags = np.abs(ref.e4m3_values(q)) @ np.abs(ref.e4m3_values(rows)).T
+        tol = tol + 2.0**-10 * (mags / by if similarity == "cosine" else mags)
     ld = n + (n % 3) * 5  # rows of the output may be longer
     out = torch.full((nq + 1, ld), 7.0, device="cuda", dtype=torch.float32 if dtype == "f32" else torch.bfloat16)
     qd = torch.from_numpy(q).cuda()

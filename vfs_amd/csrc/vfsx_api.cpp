@@ -397,7 +397,7 @@ struct vfsx_corpus {
     uint32_t small_off = 0;                                  // ... and how many such queries still skip it
 
     // probabilities over the store and the 8-bit floating point copy (vfsx_prob.hip, vfsx_f8.hip)
-    VmArray va_row_inv, va_f8, va_f8_exp; // per row: 1 / |x|; e4m3 chunks; scales
+    VmArray va_row_inv, va_row_scale, va_f8, va_f8_exp; // per row: 1 / |x|; scale of its f16 pairs; e4m3 chunks; scales
     float *d_max_norm = nullptr;          // largest finite |x| of the first prob_rows rows
     uint64_t prob_rows = 0, f8_rows = 0;  // rows that the arrays cover
     bool f8_enabled = false;
@@ -1493,6 +1493,7 @@ void vfsx_corpus_destroy(vfsx_corpus *c)
     c->prob_work.release();
     c->prob_io.release();
     c->va_row_inv.release();
+    c->va_row_scale.release();
     c->va_f8.release();
     c->va_f8_exp.release();
     if (c->d_max_norm)
@@ -1609,7 +1610,7 @@ int vfsx_corpus_storage_info(vfsx_corpus *c, uint64_t *capacity_rows, uint64_t *
     return guarded([&] {
         ready(c);
         const VmArray *all[] = {&c->va_corpus, &c->va_norms, &c->va_ids, &c->va_mirror, &c->va_rn2, &c->va_inv,
-                                &c->va_row_inv, &c->va_f8, &c->va_f8_exp};
+                                &c->va_row_inv, &c->va_row_scale, &c->va_f8, &c->va_f8_exp};
         uint64_t copied = 0, bytes = 0;
         for (const VmArray *a : all) {
             copied += a->copy_bytes;
@@ -1950,6 +1951,8 @@ void check_prob_rows(const vfsx_corpus *c)
 {
     if (c->n_rows > vfsx::kMfmaMaxRows)
         fail(VFSX_ERR_INVALID_VECTOR, "probabilities and 8-bit scores are for shards of up to " + std::to_string(vfsx::kMfmaMaxRows) + " rows");
+    if (c->dim > vfsx::kProbMaxDim)
+        fail(VFSX_ERR_INVALID_VECTOR, "probabilities and 8-bit scores are for dimensions up to " + std::to_string(vfsx::kProbMaxDim));
     if (c->dtype == VFSX_I8 && !(std::isfinite(c->scale) && c->scale != 0.0f))
         fail(VFSX_ERR_INVALID_VECTOR, "probabilities need a finite scale factor that is not zero");
 }
@@ -1961,6 +1964,7 @@ void fill_prob_store(vfsx_corpus *c, int source, vfsx::ProbStore &st)
     st.f8 = (const uint4 *)c->va_f8.base;
     st.f8_exp = (const uint32_t *)c->va_f8_exp.base;
     st.row_inv = (const float *)c->va_row_inv.base;
+    st.row_scale = (const float *)c->va_row_scale.base;
     st.max_norm = c->d_max_norm;
     st.n_rows = (uint32_t)c->n_rows;
     st.n_pieces = (uint32_t)((c->n_rows + vfsx::kPieceRows - 1u) / vfsx::kPieceRows);
@@ -1981,16 +1985,21 @@ void ensure_prob_rows(vfsx_corpus *c, bool f8, bool capturing, hipStream_t s)
     const uint64_t max_pad = prob_pad(c->max_rows);
     const uint64_t pad = prob_pad(std::max<uint64_t>(c->n_rows, 1));
     if (rows_stale) {
-        if (!c->va_row_inv.base && c->va_corpus.reserved)
+        if (!c->va_row_inv.base && c->va_corpus.reserved) {
             c->va_row_inv.init(c->device, max_pad * sizeof(float));
+            c->va_row_scale.init(c->device, max_pad * sizeof(float));
+        }
         c->va_row_inv.grow(pad * sizeof(float), c->prob_rows * sizeof(float), s);
+        if (c->dtype == VFSX_F32)
+            c->va_row_scale.grow(pad * sizeof(float), c->prob_rows * sizeof(float), s);
         if (!c->d_max_norm) {
             HIP_CHECK(hipMalloc((void **)&c->d_max_norm, sizeof(float)));
             HIP_CHECK(hipMemsetAsync(c->d_max_norm, 0, sizeof(float), s));
         }
         vfsx::ProbStore st{};
         fill_prob_store(c, VFSX_SOURCE_ROWS, st);
-        HIP_CHECK(vfsx::launch_prob_rows(st, (uint32_t)c->prob_rows, (float *)c->va_row_inv.base, c->d_max_norm, s));
+        HIP_CHECK(vfsx::launch_prob_rows(st, (uint32_t)c->prob_rows, (float *)c->va_row_inv.base,
+                                         (float *)c->va_row_scale.base, c->d_max_norm, s));
         c->prob_rows = c->n_rows;
     }
     if (f8_stale) {
@@ -2018,9 +2027,9 @@ void free_f8(vfsx_corpus *c)
 // workspaces of one round of queries, carved from c->prob_work
 struct ProbCarve {
     uint32_t round = 0, pad = 0; // queries per round; rounded up to whole tiles
-    size_t fac, eps, norm, q8, q8_exp, pieces, groups, bytes;
+    size_t fac, eps, norm, operand, q8_exp, pieces, groups, bytes;
 };
-constexpr uint32_t kProbQueryTile = 256;
+constexpr uint32_t kProbQueryTile = 128; // queries of one workgroup of the first pass, at most
 constexpr size_t kProbRoundBytes = 512u << 20; // statistics of one round of queries
 
 ProbCarve prob_carve(const vfsx_corpus *c, uint32_t nq, bool f8, bool statistics)
@@ -2042,7 +2051,7 @@ ProbCarve prob_carve(const vfsx_corpus *c, uint32_t nq, bool f8, bool statistics
     w.norm = take(w.pad * sizeof(double));
     w.fac = take(w.pad * sizeof(float));
     w.eps = take(w.pad * sizeof(float));
-    w.q8 = take(f8 ? (size_t)w.pad * vfsx::f8_chunks(c->dim) * 16u : 0);
+    w.operand = take((size_t)w.pad * (f8 ? 2u : 4u) * vfsx::query_elems(c->dim)); // bf16, or f16 pairs
     w.q8_exp = take(f8 ? (size_t)w.pad * vfsx::f8_exp_words(c->dim) * 4u : 0);
     w.pieces = take(statistics ? (size_t)w.round * n_pieces * sizeof(float4) : 0);
     w.groups = take(statistics ? (size_t)w.round * n_pieces * vfsx::kGroupsPerPiece * sizeof(float) : 0);
@@ -2062,19 +2071,20 @@ void reserve_prob_work(vfsx_corpus *c, const ProbCarve &w, bool capturing)
 }
 
 void prepare_queries(const vfsx::ProbStore &st, const ProbCarve &w, char *base, const float *d_queries, uint32_t nq, bool f8,
-                     vfsx::ProbQueries &qs, hipStream_t s)
+                     bool raw, vfsx::ProbQueries &qs, hipStream_t s)
 {
     qs.q = d_queries;
     qs.fac = (const float *)(base + w.fac);
     qs.eps = (const float *)(base + w.eps);
     qs.norm = (const double *)(base + w.norm);
-    qs.q8 = (const uint4 *)(base + w.q8);
+    qs.operand = (const uint4 *)(base + w.operand);
     qs.q8_exp = (const uint32_t *)(base + w.q8_exp);
     qs.nq = nq;
-    HIP_CHECK(vfsx::launch_prob_queries(st, d_queries, nq, (float *)(base + w.fac), (float *)(base + w.eps), (double *)(base + w.norm), s));
+    const uint32_t pad = vfsx::stream_query_pad(nq);
+    HIP_CHECK(vfsx::launch_prob_queries(st, d_queries, nq, pad, (float *)(base + w.fac), (float *)(base + w.eps), (double *)(base + w.norm),
+                                        f8 ? nullptr : (uint4 *)(base + w.operand), s));
     if (f8)
-        HIP_CHECK(vfsx::launch_f8_queries(d_queries, nq, st.dim, (nq + kProbQueryTile - 1u) / kProbQueryTile * kProbQueryTile,
-                                          (uint4 *)(base + w.q8), (uint32_t *)(base + w.q8_exp), s));
+        HIP_CHECK(vfsx::launch_f8_queries(d_queries, nq, st.dim, pad, (uint4 *)(base + w.operand), (uint32_t *)(base + w.q8_exp), raw, s));
 }
 
 void check_similarity(int similarity)
@@ -2146,7 +2156,7 @@ void log_probs_impl(vfsx_corpus *c, const LogProbsArgs &a, hipStream_t s, bool c
     for (uint32_t q0 = 0; q0 < a.nq; q0 += w.round) {
         const uint32_t qn = std::min(w.round, a.nq - q0);
         vfsx::ProbQueries qs{};
-        prepare_queries(st, w, base, a.queries + (size_t)q0 * c->dim, qn, f8, qs, s);
+        prepare_queries(st, w, base, a.queries + (size_t)q0 * c->dim, qn, f8, false, qs, s);
         float4 *pieces = (float4 *)(base + w.pieces);
         float *groups = (float *)(base + w.groups);
         HIP_CHECK(vfsx::launch_prob_pieces(st, qs, pieces, groups, s));
@@ -2185,7 +2195,7 @@ void scores_f8_impl(vfsx_corpus *c, const float *d_queries, uint32_t nq, int sim
     for (uint32_t q0 = 0; q0 < nq; q0 += w.round) {
         const uint32_t qn = std::min(w.round, nq - q0);
         vfsx::ProbQueries qs{};
-        prepare_queries(st, w, c->prob_work.p, d_queries + (size_t)q0 * c->dim, qn, true, qs, s);
+        prepare_queries(st, w, c->prob_work.p, d_queries + (size_t)q0 * c->dim, qn, true, out_dtype == VFSX_SCORES_BF16, qs, s);
         HIP_CHECK(vfsx::launch_f8_scores(st, qs, (char *)d_out + (size_t)q0 * ld * elem, ld, out_dtype == VFSX_SCORES_BF16, s));
     }
 }

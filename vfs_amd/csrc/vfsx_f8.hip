@@ -88,14 +88,18 @@ __global__ __launch_bounds__(64) void f8_rows_kernel(const uint4 *__restrict__ r
     f8_exp[((size_t)rb * words + word) * 64u + lane] = exps;
 }
 
-// Queries, row-major f32 -> the same layout.  One wave per (query, dword of four scales), two elements of a block per lane; queries
-// beyond nq become zeros (the product computes whole tiles of queries).
-__global__ __launch_bounds__(64) void f8_queries_kernel(const float *__restrict__ q, uint32_t nq, uint32_t dim, uint32_t chunks8,
-                                                        uint32_t words, uint4 *__restrict__ q8, uint32_t *__restrict__ q8_exp)
+// Queries, row-major f32 -> the operand of the product: e4m3 bytes in the layout of the rows, with their scales (raw), or the same values in
+// bf16 (8 significant bits and the exponent range of f32 hold them exactly).  One wave per (query, four blocks), two elements of a block
+// per lane; queries beyond nq become zeros (the product computes whole tiles of queries).
+template <bool RAW>
+__global__ __launch_bounds__(64) void f8_queries_kernel(const float *__restrict__ q, uint32_t nq, uint32_t dim, uint32_t blocks,
+                                                        uint32_t words, uint4 *__restrict__ operand, uint32_t *__restrict__ q8_exp)
 {
     const uint32_t lane = threadIdx.x, qi = blockIdx.x, word = blockIdx.y;
     const float *src = q + (size_t)qi * dim;
-    uint8_t *dst = (uint8_t *)(q8 + (size_t)(qi / 64u) * chunks8 * 64u + (qi & 63u));
+    // element k of a query lies in byte (value) k % 16 (8) of its chunk k / 16 (8); chunks are 1 KiB apart
+    constexpr uint32_t kPerChunk = RAW ? 16u : 8u;
+    uint8_t *dst = (uint8_t *)(operand + (size_t)(qi / 64u) * (blocks * kF8Block / kPerChunk) * 64u + (qi & 63u));
     uint32_t exps = 0;
     for (uint32_t j = 0; j < 4u; ++j) {
         const uint32_t kb = word * 4u + j, k = kb * kF8Block + 2u * lane;
@@ -106,14 +110,19 @@ __global__ __launch_bounds__(64) void f8_queries_kernel(const float *__restrict_
             top = fmaxf(top, __shfl_xor(top, o, 64));
         const int e = bad ? 0 : f8_exponent(top);
         exps |= (uint32_t)(e + 127) << (8u * j);
-        if (kb * kF8ChunksPerBlock < chunks8) {
-            const float by = pow2_neg(e);
-            const uint16_t w = bad ? (uint16_t)0x7f7f : (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(a * by, b * by, 0, false);
-            // element k of a row lies in byte k % 16 of chunk k / 16
-            *(uint16_t *)(dst + (size_t)(k / 16u) * 1024u + (k & 15u)) = w;
+        if (kb >= blocks)
+            continue;
+        const float by = pow2_neg(e);
+        const int w = bad ? 0x7f7f : __builtin_amdgcn_cvt_pk_fp8_f32(a * by, b * by, 0, false) & 0xffff;
+        if (RAW) {
+            *(uint16_t *)(dst + (size_t)(k / 16u) * 1024u + (k & 15u)) = (uint16_t)w;
+        } else {
+            typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+            const bf16x2 v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)w, __uint_as_float((uint32_t)(e + 127) << 23), false);
+            *(uint32_t *)(dst + (size_t)(k / 8u) * 1024u + (k & 7u) * 2u) = __builtin_bit_cast(uint32_t, v);
         }
     }
-    if (lane == 0)
+    if (RAW && lane == 0)
         q8_exp[((size_t)(qi / 64u) * words + word) * 64u + (qi & 63u)] = exps;
 }
 
@@ -130,23 +139,6 @@ __global__ void f8_get_rows_kernel(const uint4 *__restrict__ f8, const uint32_t 
     out[t] = ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)byte, 0), e);
 }
 
-// ---- scores, one thread per (query, row) ------------------------------------------------------------------------------------
-template <typename OUT>
-__global__ __launch_bounds__(256) void f8_scores_kernel(ProbStore st, ProbQueries qs, OUT *__restrict__ out, uint64_t ld)
-{
-    const uint32_t row = blockIdx.x * 256u + threadIdx.x, qi = blockIdx.y;
-    if (row >= st.n_rows)
-        return;
-    float s = f8_dot(st, qs, qi, row);
-    if (st.cosine) {
-        const float inv = st.row_inv[row];
-        s = qs.norm[qi] > 0.0 && inv >= 0.0f ? s * qs.fac[qi] * inv : __builtin_nanf("");
-    } else {
-        s *= qs.fac[qi];
-    }
-    out[(size_t)qi * ld + row] = (OUT)s;
-}
-
 } // namespace
 
 hipError_t launch_f8_rows(const uint4 *rows, uint32_t d_chunks, uint32_t dim, uint32_t row0, uint32_t n_rows, uint32_t n_pad,
@@ -159,9 +151,13 @@ hipError_t launch_f8_rows(const uint4 *rows, uint32_t d_chunks, uint32_t dim, ui
     return hipGetLastError();
 }
 
-hipError_t launch_f8_queries(const float *q, uint32_t nq, uint32_t dim, uint32_t nq_pad, uint4 *q8, uint32_t *q8_exp, hipStream_t s)
+hipError_t launch_f8_queries(const float *q, uint32_t nq, uint32_t dim, uint32_t nq_pad, uint4 *operand, uint32_t *q8_exp, bool raw, hipStream_t s)
 {
-    f8_queries_kernel<<<dim3(nq_pad, f8_exp_words(dim)), 64, 0, s>>>(q, nq, dim, f8_chunks(dim), f8_exp_words(dim), q8, q8_exp);
+    const dim3 grid(nq_pad, f8_exp_words(dim));
+    if (raw)
+        f8_queries_kernel<true><<<grid, 64, 0, s>>>(q, nq, dim, f8_blocks(dim), f8_exp_words(dim), operand, q8_exp);
+    else
+        f8_queries_kernel<false><<<grid, 64, 0, s>>>(q, nq, dim, f8_blocks(dim), f8_exp_words(dim), operand, q8_exp);
     return hipGetLastError();
 }
 
@@ -172,16 +168,6 @@ hipError_t launch_f8_get_rows(const uint4 *f8, const uint32_t *f8_exp, uint32_t 
     if (blocks > 0x7fffffffull)
         return hipErrorInvalidValue;
     f8_get_rows_kernel<<<(uint32_t)blocks, 256, 0, s>>>(f8, f8_exp, dim, f8_chunks(dim), f8_exp_words(dim), d_rows, n, out);
-    return hipGetLastError();
-}
-
-hipError_t launch_f8_scores(const ProbStore &st, const ProbQueries &q, void *out, uint64_t ld, int bf16, hipStream_t s)
-{
-    const dim3 grid((st.n_rows + 255u) / 256u, q.nq);
-    if (bf16)
-        f8_scores_kernel<__bf16><<<grid, 256, 0, s>>>(st, q, (__bf16 *)out, ld);
-    else
-        f8_scores_kernel<float><<<grid, 256, 0, s>>>(st, q, (float *)out, ld);
     return hipGetLastError();
 }
 

@@ -19,9 +19,9 @@ inline uint32_t f8_chunks(uint32_t dim) { return f8_blocks(dim) * kF8ChunksPerBl
 inline uint32_t f8_exp_words(uint32_t dim) { return (f8_blocks(dim) + 3u) / 4u; }
 
 // ---- log probabilities: pieces and groups -----------------------------------------------------------------------------------
-// The first pass leaves, for each query, one (max, sum, weighted sum) per PIECE of 128 rows and one maximum per GROUP of
-// 16 rows; the second pass (one workgroup per query) joins them and looks into the few groups that can hold a result.
-constexpr uint32_t kPieceRows = 128;
+// The first pass leaves, for each query, one (max, sum, weighted sum) per PIECE of 64 rows (a row-block) and one maximum per
+// GROUP of 16 rows; the second pass (one workgroup per query) joins them and looks into the few groups that can hold a result.
+constexpr uint32_t kPieceRows = 64;
 constexpr uint32_t kGroupRows = 16;
 constexpr uint32_t kGroupsPerPiece = kPieceRows / kGroupRows;
 
@@ -34,7 +34,8 @@ struct ProbStore {
     const uint4 *rows;     // rb64: f32 or int8
     const uint4 *f8;       // rb64: e4m3 (source f8)
     const uint32_t *f8_exp;
-    const float *row_inv;  // [n_rows] 1 / |x|; < 0: the row has no cosine
+    const float *row_inv;  // [whole row-blocks] 1 / |x|; < 0: the row has no cosine
+    const float *row_scale; // [whole row-blocks] f32 rows: 2^a with |x| 2^a <= 2^10, about
     const float *max_norm; // device scalar: the largest finite |x| of the store
     const float *bias;     // [n_rows] or nullptr
     uint32_t n_rows, n_pieces;
@@ -45,8 +46,8 @@ struct ProbStore {
 // the queries of one launch, prepared (prob_query_kernel)
 struct ProbQueries {
     const float *q;        // [nq][dim] as the caller gave them
-    const uint4 *q8;       // rb64 e4m3, whole row-blocks (source f8)
-    const uint32_t *q8_exp;
+    const uint4 *operand;  // whole blocks of 64 queries, 16-byte chunks as in rb64: f16 pairs (f32 and int8 rows), bf16 (f8), e4m3 (f8 raw)
+    const uint32_t *q8_exp; // f8 raw: scales, as the rows'
     const float *fac;      // [nq] logit = product * fac [* row_inv] + bias
     const float *eps;      // [nq] how far a first-pass logit may be from its value, relative to its row's part (see vfsx_prob.hip)
     const double *norm;    // [nq] |q|; 0: the query has no cosine
@@ -64,18 +65,34 @@ struct ProbFinish {
     uint32_t n_given, k;
 };
 
-hipError_t launch_prob_rows(const ProbStore &st, uint32_t row0, float *row_inv, float *max_norm, hipStream_t s);
-hipError_t launch_prob_queries(const ProbStore &st, const float *q, uint32_t nq, float *fac, float *eps, double *norm, hipStream_t s);
-hipError_t launch_prob_pieces(const ProbStore &st, const ProbQueries &q, float4 *pieces, float *groups, hipStream_t s);
+// elements of one query operand: whole blocks, which are whole K-steps of every kind
+constexpr uint32_t kQueryPad = 128;
+inline uint32_t query_elems(uint32_t dim) { return (dim + kQueryPad - 1u) / kQueryPad * kQueryPad; }
+
+hipError_t launch_prob_rows(const ProbStore &st, uint32_t row0, float *row_inv, float *row_scale, float *max_norm, hipStream_t s);
+// nq_pad: whole tiles of queries; those beyond nq become zeros.  `pairs` nullptr: only the factors (source f8)
+hipError_t launch_prob_queries(const ProbStore &st, const float *q, uint32_t nq, uint32_t nq_pad, float *fac, float *eps, double *norm,
+                               uint4 *pairs, hipStream_t s);
 hipError_t launch_prob_finish(const ProbStore &st, const ProbQueries &q, const ProbFinish &f, hipStream_t s);
+
+// vfsx_stream.hip: the first pass
+constexpr uint32_t kProbMaxDim = 1u << 20; // offsets inside a row-block and a block of queries stay below 2^31
+// queries the first pass computes for a launch of nq: whole tiles of 32, 64 or 128
+inline uint32_t stream_query_pad(uint32_t nq)
+{
+    const uint32_t tile = nq <= 32u ? 32u : (nq <= 64u ? 64u : 128u);
+    return (nq + tile - 1u) / tile * tile;
+}
+hipError_t launch_prob_pieces(const ProbStore &st, const ProbQueries &q, float4 *pieces, float *groups, hipStream_t s);
+// out[nq][ld]: f32 (bf16 = 0) or bf16
+hipError_t launch_f8_scores(const ProbStore &st, const ProbQueries &q, void *out, uint64_t ld, int bf16, hipStream_t s);
 
 // vfsx_f8.hip
 hipError_t launch_f8_rows(const uint4 *rows, uint32_t d_chunks, uint32_t dim, uint32_t row0, uint32_t n_rows, uint32_t n_pad,
                           uint4 *f8, uint32_t *f8_exp, hipStream_t s);
-hipError_t launch_f8_queries(const float *q, uint32_t nq, uint32_t dim, uint32_t nq_pad, uint4 *q8, uint32_t *q8_exp, hipStream_t s);
+// raw: e4m3 bytes and scales; otherwise the same values as bf16 (exact), no scales
+hipError_t launch_f8_queries(const float *q, uint32_t nq, uint32_t dim, uint32_t nq_pad, uint4 *operand, uint32_t *q8_exp, bool raw, hipStream_t s);
 hipError_t launch_f8_get_rows(const uint4 *f8, const uint32_t *f8_exp, uint32_t dim, const uint64_t *d_rows, uint64_t n, float *out,
                               hipStream_t s);
-// out[nq][ld]: f32 (bf16 = 0) or bf16
-hipError_t launch_f8_scores(const ProbStore &st, const ProbQueries &q, void *out, uint64_t ld, int bf16, hipStream_t s);
 
 } // namespace vfsx

@@ -31,13 +31,27 @@ namespace vfsx {
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
+// 2^a, the scale that brings vectors of norm r into the range of f16 pairs: r 2^a in (2^9, 2^10], so that elements 2^19 times smaller
+// than the norm still have a normal low half.  r = 0: 1; NaN or infinite: NaN.
+__device__ __forceinline__ float pair_scale(double r)
+{
+    if (!(r < __builtin_inf()))
+        return __builtin_nanf("");
+    if (r == 0.0)
+        return 1.0f;
+    int e;
+    (void)frexp(r, &e); // r = m 2^e, m in [0.5, 1)
+    e = 10 - e;
+    e = e > 126 ? 126 : (e < -126 ? -126 : e);
+    return __uint_as_float((uint32_t)(127 + e) << 23);
+}
 
 // ---- operands of a store: 1 / |x| per row, the largest |x| -------------------------------------------------------------------
 // One thread per row.  Norms in f64: they divide every logit.  A norm whose square is zero in f32 counts as zero.
 template <int SRC>
 __global__ __launch_bounds__(256) void prob_rows_kernel(const uint4 *__restrict__ rows, uint32_t d_chunks, uint32_t row0, uint32_t n_rows,
-                                                        float *__restrict__ row_inv, float *__restrict__ max_norm)
+                                                        float *__restrict__ row_inv, float *__restrict__ row_scale,
+                                                        float *__restrict__ max_norm)
 {
     const uint64_t row = (uint64_t)row0 + (uint64_t)blockIdx.x * 256u + threadIdx.x;
     float norm = 0.0f;
@@ -48,6 +62,8 @@ __global__ __launch_bounds__(256) void prob_rows_kernel(const uint4 *__restrict_
             s += chunk_square<SRC>(p[(size_t)c * 64u]);
         const double r = __builtin_sqrt(s);
         row_inv[row] = (float)s == 0.0f ? -1.0f : (float)(1.0 / r);
+        if (SRC == kProbF32)
+            row_scale[row] = pair_scale(r);
         norm = (float)r;
     }
     norm = norm < __builtin_inff() ? norm : 0.0f; // (a row with a NaN or an infinity has no finite logit)
@@ -58,87 +74,55 @@ __global__ __launch_bounds__(256) void prob_rows_kernel(const uint4 *__restrict_
 }
 
 // ---- queries -------------------------------------------------------------------------------------------------------------------
-__global__ __launch_bounds__(64) void prob_queries_kernel(ProbStore st, const float *__restrict__ q, float *__restrict__ fac,
-                                                          float *__restrict__ eps, double *__restrict__ norm)
+// One wave per query: its norm, its factor (logit = product * factor [/ |x|] + bias) and its f16 pairs.  Pairs lie as the rows do in rb64:
+// 64-query blocks of 1 KiB pieces, piece 2 c + part = elements 8 c .. 8 c + 7 of 64 queries, part 0 = hi, 1 = lo.
+__global__ __launch_bounds__(64) void prob_queries_kernel(ProbStore st, const float *__restrict__ q, uint32_t nq, uint32_t pair_chunks,
+                                                          float *__restrict__ fac, float *__restrict__ eps, double *__restrict__ norm,
+                                                          uint4 *__restrict__ pairs)
 {
     const uint32_t qi = blockIdx.x, lane = threadIdx.x;
+    const bool there = qi < nq;
+    const float *src = q + (size_t)qi * st.dim;
     double s = 0.0;
-    for (uint32_t j = lane; j < st.dim; j += 64u) {
-        const double v = q[(size_t)qi * st.dim + j];
-        s = __builtin_fma(v, v, s);
+    if (there) {
+        for (uint32_t j = lane; j < st.dim; j += 64u) {
+            const double v = src[j];
+            s = __builtin_fma(v, v, s);
+        }
+        for (int o = 32; o; o >>= 1)
+            s += __shfl_xor(s, o, 64);
     }
-    for (int o = 32; o; o >>= 1)
-        s += __shfl_xor(s, o, 64);
-    if (lane)
+    const double r = __builtin_sqrt(s);
+    const float scale = pair_scale(r);
+    if (pairs) {
+        uint4 *dst = pairs + (size_t)(qi / 64u) * pair_chunks * 128u + (qi & 63u);
+        for (uint32_t c = lane; c < pair_chunks; c += 64u) {
+            uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+            if (there) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) {
+                    const uint32_t k = c * 8u + i;
+                    const float x = k < st.dim ? src[k] * scale : 0.0f;
+                    const _Float16 h = (_Float16)x;
+                    const _Float16 l = (_Float16)(x - (float)h);
+                    hi[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, h) << (16u * (i & 1u));
+                    lo[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, l) << (16u * (i & 1u));
+                }
+            }
+            dst[(size_t)c * 128u] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            dst[(size_t)c * 128u + 64u] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+    }
+    if (lane || !there)
         return;
-    const double r = (float)s == 0.0f ? 0.0 : __builtin_sqrt(s);
-    norm[qi] = r;
-    if (st.cosine)
-        fac[qi] = r == 0.0 ? 0.0f : (float)(1.0 / (st.divide * r));
-    else
-        fac[qi] = (float)(1.0 / st.divide);
+    const bool zero = (float)s == 0.0f;
+    norm[qi] = zero ? 0.0 : r;
+    const double by = (pairs ? (double)scale : 1.0) * st.divide;
+    fac[qi] = (float)(1.0 / (st.cosine ? (zero ? by : by * r) : by));
     const double part = st.cosine ? 1.0 : r * (double)*st.max_norm;
     // 8-bit copies are up to 1 + 2^-4 times as long as their originals, each
     const double e = (double)(st.dim + 64u) * 0x1p-24 * (st.source == kProbF8 ? 1.25 : 1.0) * part / __builtin_fabs(st.divide);
     eps[qi] = (float)(e * (1.0 + 0x1p-20));
-}
-
-// ---- first pass, one workgroup per (piece, query), one thread per row ----------------------------------------------------------
-template <int SRC>
-__global__ __launch_bounds__(128) void prob_pieces_kernel(ProbStore st, ProbQueries qs, float4 *__restrict__ pieces, float *__restrict__ groups)
-{
-    const uint32_t piece = blockIdx.x, qi = blockIdx.y, row = piece * kPieceRows + threadIdx.x;
-    float l = neg_inf();
-    bool in = row < st.n_rows;
-    if (in) {
-        const float b = st.bias ? st.bias[row] : 0.0f;
-        in = b != neg_inf();
-        if (st.cosine)
-            in = in && st.row_inv[row] >= 0.0f && qs.norm[qi] > 0.0;
-        if (in) {
-            float v;
-            if (SRC == kProbF8) {
-                v = f8_dot(st, qs, qi, row);
-            } else {
-                const uint4 *p = st.rows + (size_t)(row >> 6) * st.d_chunks * 64u + (row & 63u);
-                const float *q = qs.q + (size_t)qi * st.dim;
-                v = 0.0f;
-                for (uint32_t c = 0; c < st.d_chunks; ++c)
-                    v = chunk_dot<SRC, float>(p[(size_t)c * 64u], q, c, st.dim, v);
-            }
-            l = v * qs.fac[qi] * (st.cosine ? st.row_inv[row] : 1.0f) + b;
-        }
-    }
-    __shared__ float part[3][2];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    float m = in ? l : neg_inf();
-    for (int o = 1; o < 16; o <<= 1)
-        m = fmaxf(m, __shfl_xor(m, o, 64));
-    if ((lane & 15u) == 0)
-        groups[((size_t)qi * st.n_pieces + piece) * kGroupsPerPiece + threadIdx.x / 16u] = m;
-    for (int o = 16; o < 64; o <<= 1)
-        m = fmaxf(m, __shfl_xor(m, o, 64));
-    if (lane == 0)
-        part[0][wave] = m;
-    __syncthreads();
-    m = fmaxf(part[0][0], part[0][1]);
-    float s = 0.0f, t = 0.0f;
-    if (in) { // (m = -inf or NaN: a logit that is not finite)
-        const float z = l - m;
-        s = exp2f(z * kLog2e);
-        t = s * z;
-    }
-    for (int o = 1; o < 64; o <<= 1) {
-        s += __shfl_xor(s, o, 64);
-        t += __shfl_xor(t, o, 64);
-    }
-    if (lane == 0) {
-        part[1][wave] = s;
-        part[2][wave] = t;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0)
-        pieces[(size_t)qi * st.n_pieces + piece] = make_float4(m, part[1][0] + part[1][1], part[2][0] + part[2][1], 0.0f);
 }
 
 // ---- second pass -----------------------------------------------------------------------------------------------------------------
@@ -174,14 +158,10 @@ __device__ double group_logit(const ProbStore &st, const ProbQueries &qs, uint32
     if (in) {
         if (SRC == kProbF8) {
             const uint4 *x = st.f8 + (size_t)(row / 64u) * st.f8_chunks * 64u + (row & 63u);
-            const uint4 *q = qs.q8 + (size_t)(qi / 64u) * st.f8_chunks * 64u + (qi & 63u);
+            const uint4 *q = qs.operand + (size_t)(qi / 64u) * st.f8_chunks * 128u + (qi & 63u);
             const uint32_t *xe = st.f8_exp + (size_t)(row / 64u) * st.f8_words * 64u + (row & 63u);
-            const uint32_t *qe = qs.q8_exp + (size_t)(qi / 64u) * st.f8_words * 64u + (qi & 63u);
-            for (uint32_t c = first; c < st.f8_chunks; c += step) {
-                const uint32_t kb = c / kF8ChunksPerBlock;
-                // (products of e4m3 values are exact in f32 and their sum over 16 of them in f64; the scale is a power of two)
-                dot += ldexp(f8_chunk_dot64(x[(size_t)c * 64u], q[(size_t)c * 64u]), f8_exp_of(xe, kb) + f8_exp_of(qe, kb));
-            }
+            for (uint32_t c = first; c < st.f8_chunks; c += step) // (e4m3 times bf16 is exact in f32, their sums in f64; a power of two scales)
+                dot += ldexp(f8_chunk_dot64(x[(size_t)c * 64u], q[(size_t)c * 128u], q[(size_t)c * 128u + 64u]), f8_exp_of(xe, c / kF8ChunksPerBlock));
         }
         if (SRC != kProbF8 || st.cosine) {
             const uint4 *p = st.rows + (size_t)(row >> 6) * st.d_chunks * 64u + (row & 63u);
@@ -258,14 +238,14 @@ __global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, 
     m = fred[0];
     for (uint32_t w = 1; w < kFinWaves; ++w)
         m = fmaxf(m, fred[w]);
-    double S = 0.0, U = 0.0;
+    double S = 0.0, U = 0.0; // over 2^(l log2e - base), exponents in units of log 2
+    const double base = piece_base64(m), L = (double)kLog2e;
     for (uint32_t i = tid; i < st.n_pieces; i += kFinThreads) {
         const float4 p = pieces[i];
         if (p.y != 0.0f) { // (0: no row of the piece is there; NaN: a logit that is not finite)
-            const float z = p.x - m;
-            const double e = (double)exp2f(z * kLog2e);
+            const double z = piece_base64(p.x) - base, e = (double)exp2f((float)z);
             S += (double)p.y * e;
-            U += ((double)p.z + (double)z * (double)p.y) * e;
+            U += e == 0.0 ? 0.0 : ((double)p.z + z * (double)p.y) * e;
         }
     }
     for (int o = 1; o < 64; o <<= 1) {
@@ -282,7 +262,7 @@ __global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, 
         S += red[0][w];
         U += red[1][w];
     }
-    const bool poisoned = !(S < __builtin_inf()) || U != U; // (S >= 1 or 0 otherwise)
+    const bool poisoned = !(S < __builtin_inf()) || U != U; // (S is about 1 or more, or 0 otherwise)
     const bool none = S == 0.0;
     const double nan = __builtin_nan("");
 
@@ -403,7 +383,7 @@ __global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, 
     if (poisoned) {
         lse = entropy = nan;
     } else if (have) {
-        const double M = best[0].l, shift = (double)m - M, by = exp(shift);
+        const double M = best[0].l, shift = base / L - M, by = exp(shift);
         double s_new = 0.0, u_new = 0.0;
         for (uint32_t j = 0; j < have; ++j) { // (every thread the same sums, in the same order)
             const uint32_t group = best[j].row / kGroupRows;
@@ -412,14 +392,19 @@ __global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, 
                 first = first && best[i].row / kGroupRows != group;
             if (!first)
                 continue;
-            const double z = best[j].l - M, e = exp(z), z1 = (double)(groups[group] - m), e1 = exp(z1);
+            const double z = best[j].l - M, e = exp(z);
             s_new += e;
             u_new += e * z;
-            S -= e1;
-            U -= e1 * z1;
+            // (the very terms that the sums have: where nothing else is there, nothing is left)
+            const float g = groups[group], pm = pieces[group / kGroupsPerPiece].x;
+            const float z1 = piece_is_huge(pm) ? (g - pm) * kLog2e : __builtin_fmaf(g, kLog2e, -piece_base(pm));
+            const float e1 = __builtin_amdgcn_exp2f(z1);
+            const double zp = piece_base64(pm) - base, ep = (double)exp2f((float)zp);
+            S -= (double)e1 * ep;
+            U -= ((double)(e1 * z1) + zp * (double)e1) * ep;
         }
         S = S > 0.0 ? S : 0.0;
-        const double total = S * by + s_new, weighted = (U + shift * S) * by + u_new;
+        const double total = S * by + s_new, weighted = (U / L + shift * S) * by + u_new;
         lse = M + log(total);
         entropy = log(total) - weighted / total;
         entropy = entropy > 0.0 ? entropy : 0.0;
@@ -462,35 +447,23 @@ __global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, 
 
 } // namespace
 
-hipError_t launch_prob_rows(const ProbStore &st, uint32_t row0, float *row_inv, float *max_norm, hipStream_t s)
+hipError_t launch_prob_rows(const ProbStore &st, uint32_t row0, float *row_inv, float *row_scale, float *max_norm, hipStream_t s)
 {
     if (st.n_rows <= row0)
         return hipSuccess;
     const uint32_t blocks = (st.n_rows - row0 + 255u) / 256u;
     if (st.source == kProbI8)
-        prob_rows_kernel<kProbI8><<<blocks, 256, 0, s>>>(st.rows, st.d_chunks, row0, st.n_rows, row_inv, max_norm);
+        prob_rows_kernel<kProbI8><<<blocks, 256, 0, s>>>(st.rows, st.d_chunks, row0, st.n_rows, row_inv, row_scale, max_norm);
     else
-        prob_rows_kernel<kProbF32><<<blocks, 256, 0, s>>>(st.rows, st.d_chunks, row0, st.n_rows, row_inv, max_norm);
+        prob_rows_kernel<kProbF32><<<blocks, 256, 0, s>>>(st.rows, st.d_chunks, row0, st.n_rows, row_inv, row_scale, max_norm);
     return hipGetLastError();
 }
 
-hipError_t launch_prob_queries(const ProbStore &st, const float *q, uint32_t nq, float *fac, float *eps, double *norm, hipStream_t s)
+hipError_t launch_prob_queries(const ProbStore &st, const float *q, uint32_t nq, uint32_t nq_pad, float *fac, float *eps, double *norm,
+                               uint4 *pairs, hipStream_t s)
 {
-    prob_queries_kernel<<<nq, 64, 0, s>>>(st, q, fac, eps, norm);
-    return hipGetLastError();
-}
-
-hipError_t launch_prob_pieces(const ProbStore &st, const ProbQueries &q, float4 *pieces, float *groups, hipStream_t s)
-{
-    if (!st.n_pieces)
-        return hipSuccess;
-    const dim3 grid(st.n_pieces, q.nq);
-    if (st.source == kProbI8)
-        prob_pieces_kernel<kProbI8><<<grid, 128, 0, s>>>(st, q, pieces, groups);
-    else if (st.source == kProbF8)
-        prob_pieces_kernel<kProbF8><<<grid, 128, 0, s>>>(st, q, pieces, groups);
-    else
-        prob_pieces_kernel<kProbF32><<<grid, 128, 0, s>>>(st, q, pieces, groups);
+    const uint32_t chunks = query_elems(st.dim) / 8u;
+    prob_queries_kernel<<<pairs ? nq_pad : nq, 64, 0, s>>>(st, q, nq, chunks, fac, eps, norm, pairs);
     return hipGetLastError();
 }
 

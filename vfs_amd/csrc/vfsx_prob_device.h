@@ -66,45 +66,32 @@ __device__ __forceinline__ T chunk_dot(uint4 v, const float *__restrict__ q, uin
     return acc;
 }
 
-__device__ __forceinline__ double f8_chunk_dot64(uint4 u, uint4 v)
+// 16 e4m3 values times 16 bf16 values
+__device__ __forceinline__ double f8_chunk_dot64(uint4 u, uint4 v0, uint4 v1)
 {
-    const uint32_t a[4] = {u.x, u.y, u.z, u.w}, b[4] = {v.x, v.y, v.z, v.w};
+    const uint32_t a[4] = {u.x, u.y, u.z, u.w}, b[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
     double s = 0.0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        s += (double)(__builtin_amdgcn_cvt_f32_fp8((int)a[i], 0) * __builtin_amdgcn_cvt_f32_fp8((int)b[i], 0));
-        s += (double)(__builtin_amdgcn_cvt_f32_fp8((int)a[i], 1) * __builtin_amdgcn_cvt_f32_fp8((int)b[i], 1));
-        s += (double)(__builtin_amdgcn_cvt_f32_fp8((int)a[i], 2) * __builtin_amdgcn_cvt_f32_fp8((int)b[i], 2));
-        s += (double)(__builtin_amdgcn_cvt_f32_fp8((int)a[i], 3) * __builtin_amdgcn_cvt_f32_fp8((int)b[i], 3));
+        const float x[4] = {__builtin_amdgcn_cvt_f32_fp8((int)a[i], 0), __builtin_amdgcn_cvt_f32_fp8((int)a[i], 1),
+                            __builtin_amdgcn_cvt_f32_fp8((int)a[i], 2), __builtin_amdgcn_cvt_f32_fp8((int)a[i], 3)};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t w = b[2 * i + j];
+            s = __builtin_fma((double)x[2 * j], (double)__uint_as_float(w << 16), s);
+            s = __builtin_fma((double)x[2 * j + 1], (double)__uint_as_float(w & 0xffff0000u), s);
+        }
     }
     return s;
 }
 
-// q8 . x8 of one row, one thread
-__device__ __forceinline__ float f8_dot(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row)
-{
-    const uint4 *x = st.f8 + (size_t)(row / 64u) * st.f8_chunks * 64u + (row & 63u);
-    const uint4 *q = qs.q8 + (size_t)(qi / 64u) * st.f8_chunks * 64u + (qi & 63u);
-    const uint32_t *xe = st.f8_exp + (size_t)(row / 64u) * st.f8_words * 64u + (row & 63u);
-    const uint32_t *qe = qs.q8_exp + (size_t)(qi / 64u) * st.f8_words * 64u + (qi & 63u);
-    float sum = 0.0f;
-    for (uint32_t kb = 0; kb < st.f8_chunks / kF8ChunksPerBlock; ++kb) {
-        float b = 0.0f;
-        for (uint32_t c = 0; c < kF8ChunksPerBlock; ++c) {
-            const uint4 u = x[(size_t)(kb * kF8ChunksPerBlock + c) * 64u], v = q[(size_t)(kb * kF8ChunksPerBlock + c) * 64u];
-            const uint32_t ux[4] = {u.x, u.y, u.z, u.w}, vx[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                b = __builtin_fmaf(__builtin_amdgcn_cvt_f32_fp8((int)ux[i], 0), __builtin_amdgcn_cvt_f32_fp8((int)vx[i], 0), b);
-                b = __builtin_fmaf(__builtin_amdgcn_cvt_f32_fp8((int)ux[i], 1), __builtin_amdgcn_cvt_f32_fp8((int)vx[i], 1), b);
-                b = __builtin_fmaf(__builtin_amdgcn_cvt_f32_fp8((int)ux[i], 2), __builtin_amdgcn_cvt_f32_fp8((int)vx[i], 2), b);
-                b = __builtin_fmaf(__builtin_amdgcn_cvt_f32_fp8((int)ux[i], 3), __builtin_amdgcn_cvt_f32_fp8((int)vx[i], 3), b);
-            }
-        }
-        sum += ldexpf(b, f8_exp_of(xe, kb) + f8_exp_of(qe, kb));
-    }
-    return sum;
-}
+// The sums of a piece are over 2^(l log2e - base), base = m log2e rounded to f32 (one fused operation per exponent); the second pass takes
+// the same base.  Beyond 1e30 the product would leave the range of f32: there the sums are over 2^((l - m) log2e).
+constexpr float kLog2e = 1.44269504088896340736f;
+__device__ __forceinline__ float piece_base(float m) { return m * kLog2e; }
+__device__ __forceinline__ bool piece_is_huge(float m) { return !(fabsf(m) < 1e30f); }
+// ... in f64, in units of log 2
+__device__ __forceinline__ double piece_base64(float m) { return piece_is_huge(m) ? (double)m * (double)kLog2e : (double)piece_base(m); }
 
 } // namespace
 } // namespace vfsx
