@@ -2027,7 +2027,7 @@ void free_f8(vfsx_corpus *c)
 // workspaces of one round of queries, carved from c->prob_work
 struct ProbCarve {
     uint32_t round = 0, pad = 0; // queries per round; rounded up to whole tiles
-    size_t fac, eps, norm, operand, q8_exp, pieces, groups, bytes;
+    size_t fac, eps, norm, operand, q8_exp, pieces, groups, units, bytes;
 };
 constexpr uint32_t kProbQueryTile = 128; // queries of one workgroup of the first pass, at most
 constexpr size_t kProbRoundBytes = 512u << 20; // statistics of one round of queries
@@ -2036,7 +2036,8 @@ ProbCarve prob_carve(const vfsx_corpus *c, uint32_t nq, bool f8, bool statistics
 {
     ProbCarve w{};
     const uint64_t n_pieces = (c->n_rows + vfsx::kPieceRows - 1u) / vfsx::kPieceRows;
-    const uint64_t per_q = n_pieces * (sizeof(float4) + vfsx::kGroupsPerPiece * sizeof(float));
+    const uint64_t n_units = vfsx::prob_units(n_pieces);
+    const uint64_t per_q = n_pieces * (sizeof(float4) + vfsx::kGroupsPerPiece * sizeof(float)) + n_units * sizeof(vfsx::ProbUnit);
     uint64_t round = 32768;
     if (statistics && per_q)
         round = std::min<uint64_t>(round, std::max<uint64_t>(kProbQueryTile, kProbRoundBytes / per_q / kProbQueryTile * kProbQueryTile));
@@ -2055,6 +2056,7 @@ ProbCarve prob_carve(const vfsx_corpus *c, uint32_t nq, bool f8, bool statistics
     w.q8_exp = take(f8 ? (size_t)w.pad * vfsx::f8_exp_words(c->dim) * 4u : 0);
     w.pieces = take(statistics ? (size_t)w.round * n_pieces * sizeof(float4) : 0);
     w.groups = take(statistics ? (size_t)w.round * n_pieces * vfsx::kGroupsPerPiece * sizeof(float) : 0);
+    w.units = take(statistics ? (size_t)w.round * n_units * sizeof(vfsx::ProbUnit) : 0);
     w.bytes = at;
     return w;
 }
@@ -2163,6 +2165,8 @@ void log_probs_impl(vfsx_corpus *c, const LogProbsArgs &a, hipStream_t s, bool c
         vfsx::ProbFinish f{};
         f.pieces = pieces;
         f.groups = groups;
+        f.units = (vfsx::ProbUnit *)(base + w.units);
+        f.n_units = vfsx::prob_units(st.n_pieces);
         f.given = a.n_given ? a.rows + (size_t)q0 * a.n_given : nullptr;
         f.log_probs = a.n_given ? a.log_probs + (size_t)q0 * a.n_given : nullptr;
         f.n_given = a.n_given;

@@ -20,9 +20,9 @@ inline uint32_t f8_exp_words(uint32_t dim) { return (f8_blocks(dim) + 3u) / 4u; 
 
 // ---- log probabilities: pieces and groups -----------------------------------------------------------------------------------
 // The first pass leaves, for each query, one (max, sum, weighted sum) per PIECE of 64 rows (a row-block) and one maximum per
-// GROUP of 16 rows; the second pass (one workgroup per query) joins them and looks into the few groups that can hold a result.
+// GROUP of 8 rows; the second pass (one workgroup per query) joins them and looks into the few groups that can hold a result.
 constexpr uint32_t kPieceRows = 64;
-constexpr uint32_t kGroupRows = 16;
+constexpr uint32_t kGroupRows = 8;
 constexpr uint32_t kGroupsPerPiece = kPieceRows / kGroupRows;
 
 enum ProbSource { kProbF32 = 0, kProbI8 = 1, kProbF8 = 2 };
@@ -54,6 +54,16 @@ struct ProbQueries {
     uint32_t nq;
 };
 
+// pieces of a long store, joined by 64: sums over 2^(l log2e - base of m)
+struct ProbUnit {
+    double s, u;
+    float m;
+    float pad[3];
+};
+// more pieces than this are joined first (below, a launch costs more than the walk it saves)
+constexpr uint32_t kJoinPieces = 8192;
+inline uint32_t prob_units(uint64_t n_pieces) { return n_pieces > kJoinPieces ? (uint32_t)((n_pieces + 63u) / 64u) : 0u; }
+
 struct ProbFinish {
     const float4 *pieces;  // [nq][n_pieces] (max, sum, weighted sum, 0)
     const float *groups;   // [nq][n_pieces * kGroupsPerPiece]
@@ -63,6 +73,8 @@ struct ProbFinish {
     vfsx_hit *top;
     uint64_t row_base, id_base;
     uint32_t n_given, k;
+    ProbUnit *units;       // [nq][n_units], n_units 0: the pieces themselves are walked
+    uint32_t n_units;
 };
 
 // elements of one query operand: whole blocks, which are whole K-steps of every kind

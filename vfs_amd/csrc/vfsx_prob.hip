@@ -3,9 +3,9 @@
 //   l_j = sim(q, x_j) / T + b_j            rows with b_j = -inf (or without a cosine) are not there at all
 //   lse = log sum_j exp(l_j),  H = -sum_j p_j log p_j,  log p_j = l_j - lse
 //
-// First pass (the store is read once, logits are never written): for each query and PIECE of 128 rows
+// First pass (the store is read once, logits are never written): for each query and PIECE of 64 rows
 //   m = max l,  s = sum exp(l - m),  t = sum exp(l - m) (l - m)
-// and for each GROUP of 16 rows its maximum.  Second pass, one workgroup per query: with M = max m
+// and for each GROUP of 8 rows its maximum.  Second pass, one workgroup per query: with M = max m
 //   S = sum s e^(m-M),  U = sum (t + (m - M) s) e^(m-M),   lse = M + log S,   H = log S - U / S
 // First-pass logits are f32 (f32-grade
 // products, f32 exponentials); the joined sums are f64.
@@ -126,10 +126,13 @@ __global__ __launch_bounds__(64) void prob_queries_kernel(ProbStore st, const fl
 }
 
 // ---- second pass -----------------------------------------------------------------------------------------------------------------
-constexpr uint32_t kFinThreads = 256;
-constexpr uint32_t kFinWaves = kFinThreads / 64;
+// What is left per query is small (16 bytes per 64 rows, 4 per 8) but serial: joined sums, then a bound, then the few groups above
+// it, then the few rows of those.  It is bound by latency for one query -- hence 1024 threads then, and loads in flight side by side -- and
+// by what the candidate groups read for a batch: k groups or a few more, each 8 rows = 128 bytes, one cache line, of every chunk.
 constexpr uint32_t kFinGroups = 1024; // candidate groups kept at once
-constexpr uint32_t kFinRows = 1024;   // candidate rows kept at once (64 groups)
+constexpr uint32_t kFinRows = 1024;   // candidate rows kept at once
+constexpr uint32_t kBuckets = 256;    // maxima that the first bound is taken from; >= VFSX_LOG_PROBS_MAX_K
+static_assert(kBuckets >= VFSX_LOG_PROBS_MAX_K, "the first bound is one of them");
 
 struct FinCand {
     double l;
@@ -137,69 +140,97 @@ struct FinCand {
     uint32_t pad;
 };
 
-// The logit of 16 rows of a group (lane & 15), in f64, on every lane; each quarter of the wave takes every fourth chunk.  Lanes whose
-// row is not there get -inf.
-template <int SRC>
-__device__ double group_logit(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t group, bool one_row, uint32_t the_row)
+__device__ __forceinline__ bool row_is_there(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row)
 {
-    // one_row: all 64 lanes share `the_row` and split its chunks
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t row = one_row ? the_row : group * kGroupRows + (lane & 15u);
-    const uint32_t first = one_row ? lane : lane >> 4, step = one_row ? 64u : 4u;
-    bool in = row < st.n_rows;
-    float b = 0.0f;
-    if (in) {
-        b = st.bias ? st.bias[row] : 0.0f;
-        in = b != neg_inf();
-        if (st.cosine)
-            in = in && st.row_inv[row] >= 0.0f && qs.norm[qi] > 0.0;
+    return row < st.n_rows && !(st.bias && st.bias[row] == neg_inf()) && !(st.cosine && (!(st.row_inv[row] >= 0.0f) || qs.norm[qi] == 0.0));
+}
+
+// q . x over chunks first, first + step, ... of one row, in f32 or f64; sq: the sum of squares too (f64, cosine)
+template <int SRC, typename T, bool SQ>
+__device__ __forceinline__ T row_dot(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row, uint32_t first, uint32_t step,
+                                     double &sq)
+{
+    T dot = 0;
+    if constexpr (SRC == kProbF8) {
+        const uint4 *x = st.f8 + (size_t)(row / 64u) * st.f8_chunks * 64u + (row & 63u);
+        const uint4 *q = qs.operand + (size_t)(qi / 64u) * st.f8_chunks * 128u + (qi & 63u);
+        const uint32_t *xe = st.f8_exp + (size_t)(row / 64u) * st.f8_words * 64u + (row & 63u);
+#pragma unroll 4
+        for (uint32_t c = first; c < st.f8_chunks; c += step)
+            dot += scaled(f8_chunk_dot<T>(x[(size_t)c * 64u], q[(size_t)c * 128u], q[(size_t)c * 128u + 64u]), f8_exp_of(xe, c / kF8ChunksPerBlock));
     }
-    double dot = 0.0, sq = 0.0;
-    if (in) {
-        if (SRC == kProbF8) {
-            const uint4 *x = st.f8 + (size_t)(row / 64u) * st.f8_chunks * 64u + (row & 63u);
-            const uint4 *q = qs.operand + (size_t)(qi / 64u) * st.f8_chunks * 128u + (qi & 63u);
-            const uint32_t *xe = st.f8_exp + (size_t)(row / 64u) * st.f8_words * 64u + (row & 63u);
-            for (uint32_t c = first; c < st.f8_chunks; c += step) // (e4m3 times bf16 is exact in f32, their sums in f64; a power of two scales)
-                dot += ldexp(f8_chunk_dot64(x[(size_t)c * 64u], q[(size_t)c * 128u], q[(size_t)c * 128u + 64u]), f8_exp_of(xe, c / kF8ChunksPerBlock));
-        }
+    if constexpr (SRC != kProbF8 || SQ) {
         if (SRC != kProbF8 || st.cosine) {
             const uint4 *p = st.rows + (size_t)(row >> 6) * st.d_chunks * 64u + (row & 63u);
             const float *q = qs.q + (size_t)qi * st.dim;
-            for (uint32_t c = first; c < st.d_chunks; c += step) {
+            constexpr uint32_t per = SRC == kProbI8 ? 16u : 4u;
+            const uint32_t full = st.dim / per; // chunks without padding
+#pragma unroll 4
+            for (uint32_t c = first; c < full; c += step) {
                 const uint4 v = p[(size_t)c * 64u];
-                if (SRC != kProbF8)
-                    dot = chunk_dot<SRC, double>(v, q, c, st.dim, dot);
-                if (st.cosine)
+                if constexpr (SRC != kProbF8)
+                    dot = chunk_dot<SRC, T>(v, q + (size_t)c * per, dot);
+                if constexpr (SQ)
+                    sq += chunk_square<SRC>(v);
+            }
+            if (full < st.d_chunks && full % step == first) {
+                const uint4 v = p[(size_t)full * 64u];
+                if constexpr (SRC != kProbF8)
+                    dot = chunk_dot_part<SRC, T>(v, q, full, st.dim, dot);
+                if constexpr (SQ)
                     sq += chunk_square<SRC>(v);
             }
         }
     }
-    if (one_row) {
-        for (int o = 1; o < 16; o <<= 1) {
-            dot += __shfl_xor(dot, o, 64);
-            sq += __shfl_xor(sq, o, 64);
-        }
-    }
-    for (int o = 16; o < 64; o <<= 1) {
-        dot += __shfl_xor(dot, o, 64);
-        sq += __shfl_xor(sq, o, 64);
-    }
-    if (!in)
+    return dot;
+}
+
+// the logit of one row in f64, by a whole wave
+template <int SRC>
+__device__ __forceinline__ double row_logit(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row)
+{
+    if (!row_is_there(st, qs, qi, row)) // (uniform)
         return -__builtin_inf();
-    return (st.cosine ? dot / (qs.norm[qi] * __builtin_sqrt(sq) * st.divide) : dot / st.divide) + (double)b;
+    double sq = 0.0, dot = row_dot<SRC, double, true>(st, qs, qi, row, threadIdx.x & 63u, 64u, sq);
+    for (int o = 1; o < 64; o <<= 1) {
+        dot += __shfl_xor(dot, o, 64);
+        if (st.cosine)
+            sq += __shfl_xor(sq, o, 64);
+    }
+    return (st.cosine ? dot / (qs.norm[qi] * __builtin_sqrt(sq) * st.divide) : dot / st.divide) + (double)(st.bias ? st.bias[row] : 0.0f);
+}
+
+// the logits of a group's 8 rows in f32, row lane & 7 on every lane; eighths of a wave take every eighth chunk.  -inf: not there
+template <int SRC>
+__device__ __forceinline__ float group_logit(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t group, float fac)
+{
+    const uint32_t lane = threadIdx.x & 63u, row = group * kGroupRows + lane % kGroupRows;
+    const bool in = row_is_there(st, qs, qi, row);
+    double unused = 0.0;
+    float dot = in ? row_dot<SRC, float, false>(st, qs, qi, row, lane / kGroupRows, 64u / kGroupRows, unused) : 0.0f;
+    for (int o = kGroupRows; o < 64; o <<= 1)
+        dot += __shfl_xor(dot, o, 64);
+    if (!in)
+        return neg_inf();
+    return dot * fac * (st.cosine ? st.row_inv[row] : 1.0f) + (st.bias ? st.bias[row] : 0.0f);
 }
 
 __device__ __forceinline__ bool cand_before(double la, uint32_t ra, double lb, uint32_t rb) { return la > lb || (la == lb && ra < rb); }
 
-// the k-th largest of n floats in LDS (n >= k >= 1), every thread gets it: rank by counting
+// the k-th largest of n floats in LDS (n >= k >= 1; room for whole float4), every thread gets it: rank by counting
+template <uint32_t THREADS>
 __device__ float kth_of(const float *v, uint32_t n, uint32_t k, float *out)
 {
-    for (uint32_t i = threadIdx.x; i < n; i += kFinThreads) {
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
         const float a = v[i];
         uint32_t before = 0;
-        for (uint32_t j = 0; j < n; ++j)
-            before += (v[j] > a || (v[j] == a && j < i)) ? 1u : 0u;
+        for (uint32_t j = 0; j < n; j += 4u) {
+            const float4 b = *(const float4 *)(v + j);
+            const float c[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (uint32_t x = 0; x < 4u; ++x)
+                before += j + x < n && (c[x] > a || (c[x] == a && j + x < i)) ? 1u : 0u;
+        }
         if (before == k - 1u)
             *out = a;
     }
@@ -209,43 +240,108 @@ __device__ float kth_of(const float *v, uint32_t n, uint32_t k, float *out)
     return r;
 }
 
-template <int SRC>
-__global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, ProbQueries qs, ProbFinish f)
+// the k first of n candidates by (logit descending, row ascending) -> best[0 .. min(n, k))
+template <uint32_t THREADS>
+__device__ void order_candidates(const FinCand *cand, uint32_t n, uint32_t k, FinCand *best)
 {
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+        const double l = cand[i].l;
+        const uint32_t r = cand[i].row;
+        uint32_t before = 0;
+        for (uint32_t j = 0; j < n; ++j)
+            before += cand_before(cand[j].l, cand[j].row, l, r) ? 1u : 0u;
+        if (before < k)
+            best[before].l = l, best[before].row = r;
+    }
+    __syncthreads();
+}
+
+// Long stores: 64 pieces (4096 rows) joined into one unit, one wave each, so that the second pass walks 64 times less.
+__global__ __launch_bounds__(256) void prob_join_kernel(const float4 *__restrict__ pieces, uint32_t n_pieces, uint32_t n_units,
+                                                        ProbUnit *__restrict__ units)
+{
+    const uint32_t unit = blockIdx.x * 4u + (threadIdx.x >> 6), qi = blockIdx.y, lane = threadIdx.x & 63u, i = unit * 64u + lane;
+    if (unit >= n_units)
+        return;
+    const float4 p = i < n_pieces ? pieces[(size_t)qi * n_pieces + i] : make_float4(neg_inf(), 0.0f, 0.0f, 0.0f);
+    float m = p.x;
+    for (int o = 1; o < 64; o <<= 1)
+        m = fmaxf(m, __shfl_xor(m, o, 64));
+    double s = 0.0, u = 0.0;
+    add_unit(m, p.x, (double)p.y, (double)p.z, s, u);
+    for (int o = 1; o < 64; o <<= 1) {
+        s += __shfl_xor(s, o, 64);
+        u += __shfl_xor(u, o, 64);
+    }
+    if (lane == 0) {
+        ProbUnit r;
+        r.s = s;
+        r.u = u;
+        r.m = m;
+        r.pad[0] = r.pad[1] = r.pad[2] = 0;
+        units[(size_t)qi * n_units + unit] = r;
+    }
+}
+
+template <int SRC, bool JOINED, uint32_t THREADS>
+__global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, ProbQueries qs, ProbFinish f)
+{
+    constexpr uint32_t WAVES = THREADS / 64u;
     const uint32_t qi = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     const float4 *pieces = f.pieces + (size_t)qi * st.n_pieces;
     const float *groups = f.groups + (size_t)qi * st.n_pieces * kGroupsPerPiece;
+    const ProbUnit *units = f.units + (size_t)qi * f.n_units;
+    const uint32_t n_units = JOINED ? f.n_units : st.n_pieces;
+    auto unit_max = [&](uint32_t i) { return JOINED ? units[i].m : pieces[i].x; };
 
-    __shared__ double red[2][kFinWaves];
-    __shared__ float fred[kFinWaves];
-    __shared__ float lv[kFinGroups];      // maxima: of the threads' shares, then of the candidate groups
-    __shared__ uint32_t lg[kFinGroups];   // candidate groups
+    __shared__ double red[2][WAVES];
+    __shared__ float fred[WAVES];
+    __shared__ __align__(16) float lv[kFinGroups]; // maxima: of the buckets, then of the candidate groups
+    __shared__ uint32_t lg[kFinGroups];            // candidate groups
+    __shared__ uint32_t lu[kFinGroups];            // candidate units; then candidate rows
     __shared__ FinCand cand[kFinRows + VFSX_LOG_PROBS_MAX_K];
     __shared__ FinCand best[VFSX_LOG_PROBS_MAX_K];
-    __shared__ uint32_t n_lg, n_cand;
+    __shared__ uint32_t n_lu, n_lg, n_rows, n_cand;
     __shared__ float kth;
 
     // ---- M, S, U ------------------------------------------------------------------------------------------------------------
     float m = neg_inf();
-    for (uint32_t i = tid; i < st.n_pieces; i += kFinThreads)
-        m = fmaxf(m, pieces[i].x);
+#pragma unroll 4
+    for (uint32_t i = tid; i < n_units; i += THREADS)
+        m = fmaxf(m, unit_max(i));
     const float my_max = m;
     for (int o = 1; o < 64; o <<= 1)
         m = fmaxf(m, __shfl_xor(m, o, 64));
     if (lane == 0)
         fred[wave] = m;
+    if (tid == 0)
+        n_lu = n_lg = n_rows = n_cand = 0;
+    if (THREADS > kBuckets && tid < kBuckets)
+        lv[tid] = neg_inf();
     __syncthreads();
+    if (THREADS == kBuckets) {
+        lv[tid] = my_max;
+    } else {
+        // a thread's share joins bucket tid % kBuckets: the waves of one residue one after another
+        for (uint32_t r = 0; r < THREADS / kBuckets; ++r) {
+            if (tid / kBuckets == r)
+                lv[tid % kBuckets] = fmaxf(lv[tid % kBuckets], my_max);
+            __syncthreads();
+        }
+    }
     m = fred[0];
-    for (uint32_t w = 1; w < kFinWaves; ++w)
+    for (uint32_t w = 1; w < WAVES; ++w)
         m = fmaxf(m, fred[w]);
     double S = 0.0, U = 0.0; // over 2^(l log2e - base), exponents in units of log 2
     const double base = piece_base64(m), L = (double)kLog2e;
-    for (uint32_t i = tid; i < st.n_pieces; i += kFinThreads) {
-        const float4 p = pieces[i];
-        if (p.y != 0.0f) { // (0: no row of the piece is there; NaN: a logit that is not finite)
-            const double z = piece_base64(p.x) - base, e = (double)exp2f((float)z);
-            S += (double)p.y * e;
-            U += e == 0.0 ? 0.0 : ((double)p.z + z * (double)p.y) * e;
+#pragma unroll 4
+    for (uint32_t i = tid; i < n_units; i += THREADS) {
+        if (JOINED) {
+            const ProbUnit p = units[i];
+            add_unit(m, p.m, p.s, p.u, S, U);
+        } else {
+            const float4 p = pieces[i];
+            add_unit(m, p.x, (double)p.y, (double)p.z, S, U);
         }
     }
     for (int o = 1; o < 64; o <<= 1) {
@@ -258,7 +354,7 @@ __global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, 
     }
     __syncthreads();
     S = red[0][0], U = red[1][0];
-    for (uint32_t w = 1; w < kFinWaves; ++w) {
+    for (uint32_t w = 1; w < WAVES; ++w) {
         S += red[0][w];
         U += red[1][w];
     }
@@ -270,67 +366,88 @@ __global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, 
     const uint32_t k = f.k ? f.k : 1u;
     uint32_t have = 0; // rows in best[], ordered
     if (!poisoned && !none) {
-        // a first bound: the k-th largest of the threads' maxima (k <= kFinThreads pieces or more reach it)
-        lv[tid] = my_max;
+        const float eps2 = 2.0f * qs.eps[qi];
+        // first-pass logits that can be among the true k largest when `kth` is the k-th largest of some of them
+        auto below = [&](float kth_value) {
+            return kth_value == neg_inf() ? kth_value : kth_value - eps2 - 0x1p-21f * fmaxf(fabsf(kth_value), fabsf(m));
+        };
+        // a first bound: the k-th largest of the buckets' maxima, which k groups at least reach
+        float thr = below(kth_of<THREADS>(lv, kBuckets, k, &kth));
+        // units above it -> pieces -> groups
+        for (uint32_t i = tid; i < n_units; i += THREADS) {
+            const float v = unit_max(i);
+            if (v >= thr && v != neg_inf()) {
+                const uint32_t at = atomicAdd(&n_lu, 1u);
+                if (at < kFinGroups)
+                    lu[at] = i;
+            }
+        }
         __syncthreads();
-        const float bound = kth_of(lv, kFinThreads, k, &kth);
-        float thr = bound - 2.0f * qs.eps[qi] - 0x1p-21f * fmaxf(fabsf(bound), fabsf(m));
-        if (bound == neg_inf())
-            thr = neg_inf();
-        if (tid == 0)
-            n_lg = 0, n_cand = 0;
-        __syncthreads();
-        for (uint32_t i = tid; i < st.n_pieces; i += kFinThreads) {
-            if (!(pieces[i].x >= thr) || pieces[i].x == neg_inf())
-                continue;
-            for (uint32_t g = 0; g < kGroupsPerPiece; ++g) {
-                const float v = groups[(size_t)i * kGroupsPerPiece + g];
+        bool whole = n_lu <= kFinGroups;
+        if (whole) {
+            auto push_group = [&](uint32_t group, float v) {
                 if (v >= thr && v != neg_inf()) {
                     const uint32_t at = atomicAdd(&n_lg, 1u);
                     if (at < kFinGroups) {
                         lv[at] = v;
-                        lg[at] = i * kGroupsPerPiece + g;
+                        lg[at] = group;
                     }
                 }
-            }
-        }
-        __syncthreads();
-        bool whole = n_lg <= kFinGroups;
-        if (whole) {
-            const uint32_t n = n_lg;
-            if (n > k) { // the k-th largest group maximum: a closer bound
-                const float g = kth_of(lv, n, k, &kth);
-                thr = fmaxf(thr, g - 2.0f * qs.eps[qi] - 0x1p-21f * fmaxf(fabsf(g), fabsf(m)));
-            }
-            for (uint32_t i = wave; i < n; i += kFinWaves) {
-                if (!(lv[i] >= thr))
-                    continue;
-                const double l = group_logit<SRC>(st, qs, qi, lg[i], false, 0);
-                if (lane < 16u && l >= (double)thr && l != -__builtin_inf()) {
-                    const uint32_t at = atomicAdd(&n_cand, 1u);
-                    if (at < kFinRows)
-                        cand[at].l = l, cand[at].row = lg[i] * kGroupRows + lane;
+            };
+            const uint32_t n = n_lu;
+            if (JOINED) { // a wave looks through the 64 pieces of a unit
+                for (uint32_t j = wave; j < n; j += WAVES) {
+                    const uint32_t piece = lu[j] * 64u + lane;
+                    uint64_t todo = __ballot(piece < st.n_pieces && pieces[min(piece, st.n_pieces - 1u)].x >= thr);
+                    for (; todo; todo &= todo - 1u) {
+                        const uint32_t p = lu[j] * 64u + (uint32_t)__ffsll((unsigned long long)todo) - 1u;
+                        if (lane < kGroupsPerPiece)
+                            push_group(p * kGroupsPerPiece + lane, groups[(size_t)p * kGroupsPerPiece + lane]);
+                    }
+                }
+            } else {
+                for (uint32_t j = tid; j < n * kGroupsPerPiece; j += THREADS) {
+                    const uint32_t group = lu[j / kGroupsPerPiece] * kGroupsPerPiece + j % kGroupsPerPiece;
+                    push_group(group, groups[group]);
                 }
             }
             __syncthreads();
-            whole = n_cand <= kFinRows;
+            whole = n_lg <= kFinGroups;
         }
         if (whole) {
-            const uint32_t n = n_cand;
-            for (uint32_t i = tid; i < n; i += kFinThreads) {
-                const double l = cand[i].l;
-                const uint32_t r = cand[i].row;
-                uint32_t before = 0;
-                for (uint32_t j = 0; j < n; ++j)
-                    before += cand_before(cand[j].l, cand[j].row, l, r) ? 1u : 0u;
-                if (before < k)
-                    best[before].l = l, best[before].row = r;
+            const uint32_t n = n_lg;
+            if (n > k) // the k-th largest group maximum: a closer bound
+                thr = fmaxf(thr, below(kth_of<THREADS>(lv, n, k, &kth)));
+            // their rows: logits in f32 (as good as the first pass') first, then those that are left in f64
+            const float fac = (float)(st.cosine ? 1.0 / (qs.norm[qi] * st.divide) : 1.0 / st.divide);
+            for (uint32_t i = wave; i < n; i += WAVES) {
+                if (!(lv[i] >= thr))
+                    continue;
+                const float l = group_logit<SRC>(st, qs, qi, lg[i], fac);
+                if (lane < kGroupRows && l >= thr && l != neg_inf()) {
+                    const uint32_t at = atomicAdd(&n_rows, 1u);
+                    if (at < kFinRows)
+                        lu[at] = lg[i] * kGroupRows + lane;
+                }
             }
-            have = min(n, k);
             __syncthreads();
-        } else {
+            whole = n_rows <= kFinRows;
+            if (whole) {
+                const uint32_t r = n_rows;
+                for (uint32_t i = wave; i < r; i += WAVES) {
+                    const double l = row_logit<SRC>(st, qs, qi, lu[i]);
+                    if (lane == 0)
+                        cand[i].l = l, cand[i].row = lu[i];
+                }
+                __syncthreads();
+                order_candidates<THREADS>(cand, r, k, best);
+                have = min(r, k);
+            }
+        }
+        if (!whole) {
             // More near ties than fit (a store that holds one vector very often): walk the groups in order, 64 at a time, and join
             // what can displace the k-th best so far.  Equal rows that come later cannot, so they cost their logits only.
+            __syncthreads();
             const uint32_t n_groups = st.n_pieces * kGroupsPerPiece;
             for (uint32_t g0 = 0; g0 < n_groups; g0 += 64u) {
                 const float v = g0 + lane < n_groups ? groups[g0 + lane] : neg_inf();
@@ -342,35 +459,27 @@ __global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, 
                     n_cand = 0;
                 __syncthreads();
                 for (uint32_t i = 0; todo; ++i, todo &= todo - 1u) {
-                    if (i % kFinWaves != wave)
+                    if (i % WAVES != wave)
                         continue;
                     const uint32_t group = g0 + (uint32_t)__ffsll((unsigned long long)todo) - 1u;
-                    const double l = group_logit<SRC>(st, qs, qi, group, false, 0);
-                    const uint32_t r = group * kGroupRows + lane;
-                    if (lane < 16u && l != -__builtin_inf() && (have < k || cand_before(l, r, best[k - 1u].l, best[k - 1u].row))) {
-                        const uint32_t at = atomicAdd(&n_cand, 1u); // at most 64 groups of 16 rows
-                        cand[at].l = l, cand[at].row = r;
+                    for (uint32_t j = 0; j < kGroupRows; ++j) {
+                        const uint32_t r = group * kGroupRows + j;
+                        const double l = row_logit<SRC>(st, qs, qi, r);
+                        if (lane == 0 && l != -__builtin_inf() && (have < k || cand_before(l, r, best[k - 1u].l, best[k - 1u].row))) {
+                            const uint32_t at = atomicAdd(&n_cand, 1u); // at most 64 groups of 8 rows
+                            cand[at].l = l, cand[at].row = r;
+                        }
                     }
                 }
                 __syncthreads();
                 const uint32_t fresh = n_cand;
                 if (!fresh)
                     continue;
-                for (uint32_t i = tid; i < have; i += kFinThreads)
+                for (uint32_t i = tid; i < have; i += THREADS)
                     cand[fresh + i] = best[i];
                 __syncthreads();
-                const uint32_t all = fresh + have;
-                for (uint32_t i = tid; i < all; i += kFinThreads) {
-                    const double l = cand[i].l;
-                    const uint32_t r = cand[i].row;
-                    uint32_t before = 0;
-                    for (uint32_t j = 0; j < all; ++j)
-                        before += cand_before(cand[j].l, cand[j].row, l, r) ? 1u : 0u;
-                    if (before < k)
-                        best[before].l = l, best[before].row = r;
-                }
-                have = min(all, k);
-                __syncthreads();
+                order_candidates<THREADS>(cand, fresh + have, k, best);
+                have = min(fresh + have, k);
             }
         }
     }
@@ -385,23 +494,42 @@ __global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, 
     } else if (have) {
         const double M = best[0].l, shift = base / L - M, by = exp(shift);
         double s_new = 0.0, u_new = 0.0;
-        for (uint32_t j = 0; j < have; ++j) { // (every thread the same sums, in the same order)
-            const uint32_t group = best[j].row / kGroupRows;
-            bool first = true;
-            for (uint32_t i = 0; i < j; ++i)
-                first = first && best[i].row / kGroupRows != group;
-            if (!first)
-                continue;
-            const double z = best[j].l - M, e = exp(z);
+        for (uint32_t j0 = 0; j0 < have; j0 += 64u) { // (every wave the same sums, in the same order)
+            const uint32_t j = j0 + lane;
+            double e = 0.0, ez = 0.0, s1 = 0.0, u1 = 0.0;
+            if (j < have) {
+                const uint32_t group = best[j].row / kGroupRows;
+                bool first = true;
+                for (uint32_t i = 0; i < j; ++i)
+                    first = first && best[i].row / kGroupRows != group;
+                if (first) {
+                    const double z = best[j].l - M;
+                    e = exp(z);
+                    ez = e * z;
+                    // (the very terms that the sums have: where nothing else is there, nothing is left)
+                    const float g = groups[group], pm = pieces[group / kGroupsPerPiece].x;
+                    const float z1 = piece_is_huge(pm) ? (g - pm) * kLog2e : __builtin_fmaf(g, kLog2e, -piece_base(pm));
+                    const float e1 = __builtin_amdgcn_exp2f(z1);
+                    if (JOINED) {
+                        double s0 = 0.0, u0 = 0.0;
+                        const float um = units[group / kGroupsPerPiece / 64u].m;
+                        add_unit(um, pm, (double)e1, (double)(e1 * z1), s0, u0);
+                        add_unit(m, um, s0, u0, s1, u1);
+                    } else {
+                        add_unit(m, pm, (double)e1, (double)(e1 * z1), s1, u1);
+                    }
+                }
+            }
+            for (int o = 1; o < 64; o <<= 1) {
+                e += __shfl_xor(e, o, 64);
+                ez += __shfl_xor(ez, o, 64);
+                s1 += __shfl_xor(s1, o, 64);
+                u1 += __shfl_xor(u1, o, 64);
+            }
             s_new += e;
-            u_new += e * z;
-            // (the very terms that the sums have: where nothing else is there, nothing is left)
-            const float g = groups[group], pm = pieces[group / kGroupsPerPiece].x;
-            const float z1 = piece_is_huge(pm) ? (g - pm) * kLog2e : __builtin_fmaf(g, kLog2e, -piece_base(pm));
-            const float e1 = __builtin_amdgcn_exp2f(z1);
-            const double zp = piece_base64(pm) - base, ep = (double)exp2f((float)zp);
-            S -= (double)e1 * ep;
-            U -= ((double)(e1 * z1) + zp * (double)e1) * ep;
+            u_new += ez;
+            S -= s1;
+            U -= u1;
         }
         S = S > 0.0 ? S : 0.0;
         const double total = S * by + s_new, weighted = (U / L + shift * S) * by + u_new;
@@ -416,18 +544,18 @@ __global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, 
             f.entropy[qi] = (float)entropy;
     }
 
-    // ---- given rows, one wave each --------------------------------------------------------------------------------------------
+    // ---- given rows, one wave each; the most probable rows ---------------------------------------------------------------------------
     if (f.log_probs) {
-        for (uint32_t g = wave; g < f.n_given; g += kFinWaves) {
+        for (uint32_t g = wave; g < f.n_given; g += WAVES) {
             const uint64_t at = f.given[(size_t)qi * f.n_given + g] - f.row_base; // (below row_base: wraps beyond n_rows)
             double l = -__builtin_inf();
             if (at < st.n_rows)
-                l = group_logit<SRC>(st, qs, qi, 0, true, (uint32_t)at);
+                l = row_logit<SRC>(st, qs, qi, (uint32_t)at);
             if (lane == 0)
                 f.log_probs[(size_t)qi * f.n_given + g] = poisoned ? (float)nan : (l == -__builtin_inf() ? neg_inf() : (float)(l - lse));
         }
     }
-    for (uint32_t j = tid; j < f.k; j += kFinThreads) {
+    for (uint32_t j = tid; j < f.k; j += THREADS) {
         vfsx_hit h;
         if (j < have) {
             const uint32_t r = best[j].row;
@@ -441,8 +569,29 @@ __global__ __launch_bounds__(kFinThreads) void prob_finish_kernel(ProbStore st, 
             h.row = ~0ull;
             h.id = ~0ull;
         }
-        f.top[(size_t)qi * k + j] = h;
+        f.top[(size_t)qi * f.k + j] = h;
     }
+}
+
+template <int SRC>
+hipError_t finish_for(const ProbStore &st, const ProbQueries &q, const ProbFinish &f, hipStream_t s)
+{
+    // few queries leave CUs idle: more waves for each
+    const bool joined = f.n_units != 0, wide = q.nq <= 64u;
+    if (joined) {
+        prob_join_kernel<<<dim3((f.n_units + 3u) / 4u, q.nq), 256, 0, s>>>(f.pieces, st.n_pieces, f.n_units, f.units);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess)
+            return e;
+    }
+    if (wide && joined)
+        prob_finish_kernel<SRC, true, 1024><<<q.nq, 1024, 0, s>>>(st, q, f);
+    else if (wide)
+        prob_finish_kernel<SRC, false, 1024><<<q.nq, 1024, 0, s>>>(st, q, f);
+    else if (joined)
+        prob_finish_kernel<SRC, true, 256><<<q.nq, 256, 0, s>>>(st, q, f);
+    else
+        prob_finish_kernel<SRC, false, 256><<<q.nq, 256, 0, s>>>(st, q, f);
+    return hipGetLastError();
 }
 
 } // namespace
@@ -470,12 +619,10 @@ hipError_t launch_prob_queries(const ProbStore &st, const float *q, uint32_t nq,
 hipError_t launch_prob_finish(const ProbStore &st, const ProbQueries &q, const ProbFinish &f, hipStream_t s)
 {
     if (st.source == kProbI8)
-        prob_finish_kernel<kProbI8><<<q.nq, kFinThreads, 0, s>>>(st, q, f);
-    else if (st.source == kProbF8)
-        prob_finish_kernel<kProbF8><<<q.nq, kFinThreads, 0, s>>>(st, q, f);
-    else
-        prob_finish_kernel<kProbF32><<<q.nq, kFinThreads, 0, s>>>(st, q, f);
-    return hipGetLastError();
+        return finish_for<kProbI8>(st, q, f, s);
+    if (st.source == kProbF8)
+        return finish_for<kProbF8>(st, q, f, s);
+    return finish_for<kProbF32>(st, q, f, s);
 }
 
 } // namespace vfsx

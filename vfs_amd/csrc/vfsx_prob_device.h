@@ -43,34 +43,45 @@ __device__ __forceinline__ double chunk_square(uint4 v)
     }
 }
 
-// acc + chunk c of a row times the same elements of q (row-major, dim elements; stored chunks are zero beyond dim)
+// acc + a whole stored chunk times the same elements of the query (q: anywhere; 16-byte loads need no more than the 4 bytes' alignment)
 template <int SRC, typename T>
-__device__ __forceinline__ T chunk_dot(uint4 v, const float *__restrict__ q, uint32_t c, uint32_t dim, T acc)
+__device__ __forceinline__ T chunk_dot(uint4 v, const float *__restrict__ q, T acc)
 {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    if constexpr (SRC == kProbI8) {
+    constexpr int kVec = SRC == kProbI8 ? 4 : 1;
 #pragma unroll
-        for (uint32_t i = 0; i < 16u; ++i) {
-            const uint32_t k = c * 16u + i;
-            if (k < dim)
-                acc = fma_of((T)i8_at(w[i >> 2], i & 3), (T)q[k], acc);
-        }
-    } else {
+    for (int j = 0; j < kVec; ++j) {
+        float a[4];
+        __builtin_memcpy(a, q + 4 * j, 16);
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-            const uint32_t k = c * 4u + i;
-            if (k < dim)
-                acc = fma_of((T)__uint_as_float(w[i]), (T)q[k], acc);
-        }
+        for (int i = 0; i < 4; ++i)
+            acc = fma_of(SRC == kProbI8 ? (T)i8_at(w[j], i) : (T)__uint_as_float(w[i]), (T)a[i], acc);
     }
     return acc;
 }
 
+// the same for chunk c when it is a row's last and not whole: the query has nothing beyond dim
+template <int SRC, typename T>
+__device__ __forceinline__ T chunk_dot_part(uint4 v, const float *__restrict__ q, uint32_t c, uint32_t dim, T acc)
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    constexpr uint32_t per = SRC == kProbI8 ? 16u : 4u;
+#pragma unroll
+    for (uint32_t i = 0; i < per; ++i)
+        if (c * per + i < dim)
+            acc = fma_of(SRC == kProbI8 ? (T)i8_at(w[i >> 2], i & 3) : (T)__uint_as_float(w[i & 3]), (T)q[c * per + i], acc);
+    return acc;
+}
+
+__device__ __forceinline__ float scaled(float v, int e) { return ldexpf(v, e); }
+__device__ __forceinline__ double scaled(double v, int e) { return ldexp(v, e); }
+
 // 16 e4m3 values times 16 bf16 values
-__device__ __forceinline__ double f8_chunk_dot64(uint4 u, uint4 v0, uint4 v1)
+template <typename T>
+__device__ __forceinline__ T f8_chunk_dot(uint4 u, uint4 v0, uint4 v1)
 {
     const uint32_t a[4] = {u.x, u.y, u.z, u.w}, b[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-    double s = 0.0;
+    T s = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float x[4] = {__builtin_amdgcn_cvt_f32_fp8((int)a[i], 0), __builtin_amdgcn_cvt_f32_fp8((int)a[i], 1),
@@ -78,8 +89,8 @@ __device__ __forceinline__ double f8_chunk_dot64(uint4 u, uint4 v0, uint4 v1)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const uint32_t w = b[2 * i + j];
-            s = __builtin_fma((double)x[2 * j], (double)__uint_as_float(w << 16), s);
-            s = __builtin_fma((double)x[2 * j + 1], (double)__uint_as_float(w & 0xffff0000u), s);
+            s = fma_of((T)x[2 * j], (T)__uint_as_float(w << 16), s);
+            s = fma_of((T)x[2 * j + 1], (T)__uint_as_float(w & 0xffff0000u), s);
         }
     }
     return s;
@@ -92,6 +103,16 @@ __device__ __forceinline__ float piece_base(float m) { return m * kLog2e; }
 __device__ __forceinline__ bool piece_is_huge(float m) { return !(fabsf(m) < 1e30f); }
 // ... in f64, in units of log 2
 __device__ __forceinline__ double piece_base64(float m) { return piece_is_huge(m) ? (double)m * (double)kLog2e : (double)piece_base(m); }
+
+// adds sums (s, u) over the base of m_part to sums over the base of m; s = 0: nothing there, NaN: a logit that is not finite
+__device__ __forceinline__ void add_unit(float m, float m_part, double s, double u, double &S, double &U)
+{
+    if (s == 0.0)
+        return;
+    const double z = piece_base64(m_part) - piece_base64(m), e = (double)exp2f((float)z);
+    S += s * e;
+    U += e == 0.0 ? 0.0 : (u + z * s) * e;
+}
 
 } // namespace
 } // namespace vfsx

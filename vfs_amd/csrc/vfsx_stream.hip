@@ -349,7 +349,7 @@ __global__ __launch_bounds__(WAVES * 64, NT == 4 ? 2 : (NT == 2 ? 3 : 4)) void s
             const uint32_t qi = q0 + nt * 32u;
             const bool mine = qi < qs.nq;
             const float fac = mine ? qs.fac[qi] : 0.0f;
-            float top[2] = {neg_inf(), neg_inf()}, s = 0.0f, t = 0.0f, m;
+            float top[2][2] = {{neg_inf(), neg_inf()}, {neg_inf(), neg_inf()}}, s = 0.0f, t = 0.0f, m;
             auto logit = [&](uint32_t mt, uint32_t i) { // (the same address in all lanes of a half)
                 const uint32_t at = mt * 32u + h * 16u + i;
                 return __builtin_fmaf(acc[mt][nt][i], fac * row_mul[wave][at], row_add[wave][at]);
@@ -361,9 +361,9 @@ __global__ __launch_bounds__(WAVES * 64, NT == 4 ? 2 : (NT == 2 ? 3 : 4)) void s
 #pragma unroll
                     for (uint32_t i = 0; i < 16u; ++i) {
                         acc[mt][nt][i] = logit(mt, i);
-                        top[mt] = fmaxf(top[mt], acc[mt][nt][i]);
+                        top[mt][i >> 3] = fmaxf(top[mt][i >> 3], acc[mt][nt][i]);
                     }
-                m = fmaxf(top[0], top[1]);
+                m = fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[1][0], top[1][1]));
                 m = fmaxf(m, __shfl_xor(m, 32, 64));
                 const float base = piece_base(m);
 #pragma unroll
@@ -380,9 +380,9 @@ __global__ __launch_bounds__(WAVES * 64, NT == 4 ? 2 : (NT == 2 ? 3 : 4)) void s
 #pragma unroll
                     for (uint32_t i = 0; i < 16u; ++i) {
                         acc[mt][nt][i] = is_gone(mt, i) ? neg_inf() : logit(mt, i);
-                        top[mt] = fmaxf(top[mt], acc[mt][nt][i]);
+                        top[mt][i >> 3] = fmaxf(top[mt][i >> 3], acc[mt][nt][i]);
                     }
-                m = fmaxf(top[0], top[1]);
+                m = fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[1][0], top[1][1]));
                 m = fmaxf(m, __shfl_xor(m, 32, 64));
                 const float base = piece_base(m);
                 const bool huge = piece_is_huge(m);
@@ -401,13 +401,16 @@ __global__ __launch_bounds__(WAVES * 64, NT == 4 ? 2 : (NT == 2 ? 3 : 4)) void s
             s += __shfl_xor(s, 32, 64);
             t += __shfl_xor(t, 32, 64);
             if (st.cosine && mine && qs.norm[qi] == 0.0) { // no cosine: no row is there
-                m = top[0] = top[1] = neg_inf();
+                m = top[0][0] = top[0][1] = top[1][0] = top[1][1] = neg_inf();
                 s = t = 0.0f;
             }
-            const float other0 = __shfl_xor(top[0], 32, 64), other1 = __shfl_xor(top[1], 32, 64);
-            if (mine && h == 0u) {
-                out.pieces[(size_t)qi * st.n_pieces + rb] = make_float4(m, s, t, 0.0f);
-                *(float4 *)(out.groups + ((size_t)qi * st.n_pieces + rb) * kGroupsPerPiece) = make_float4(top[0], other0, top[1], other1);
+            if (mine) {
+                const size_t piece = (size_t)qi * st.n_pieces + rb;
+                if (h == 0u)
+                    out.pieces[piece] = make_float4(m, s, t, 0.0f);
+                float2 *g = (float2 *)(out.groups + piece * kGroupsPerPiece); // groups 4 mt + 2 h, + 1
+                g[h] = make_float2(top[0][0], top[0][1]);
+                g[2u + h] = make_float2(top[1][0], top[1][1]);
             }
         }
     } else {
