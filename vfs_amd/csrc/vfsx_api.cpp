@@ -2072,7 +2072,8 @@ void reserve_prob_work(vfsx_corpus *c, const ProbCarve &w, bool capturing)
     c->prob_work.reserve(w.bytes);
 }
 
-void prepare_queries(const vfsx::ProbStore &st, const ProbCarve &w, char *base, const float *d_queries, uint32_t nq, bool f8,
+// whether the first pass is the one for a few queries
+bool prepare_queries(const vfsx::ProbStore &st, const ProbCarve &w, char *base, const float *d_queries, uint32_t nq, bool f8,
                      bool raw, vfsx::ProbQueries &qs, hipStream_t s)
 {
     qs.q = d_queries;
@@ -2082,11 +2083,20 @@ void prepare_queries(const vfsx::ProbStore &st, const ProbCarve &w, char *base, 
     qs.operand = (const uint4 *)(base + w.operand);
     qs.q8_exp = (const uint32_t *)(base + w.q8_exp);
     qs.nq = nq;
+    qs.fac_out = (float *)(base + w.fac);
+    qs.eps_out = (float *)(base + w.eps);
+    qs.norm_out = (double *)(base + w.norm);
+    qs.operand_out = (uint4 *)(base + w.operand);
+    if (vfsx::few_takes(nq, st.dim, st.source)) { // the first pass prepares them itself
+        qs.operand_chunk = vfsx::few_places(nq);
+        return true;
+    }
+    qs.operand_chunk = 64;
     const uint32_t pad = vfsx::stream_query_pad(nq);
-    HIP_CHECK(vfsx::launch_prob_queries(st, d_queries, nq, pad, (float *)(base + w.fac), (float *)(base + w.eps), (double *)(base + w.norm),
-                                        f8 ? nullptr : (uint4 *)(base + w.operand), s));
+    HIP_CHECK(vfsx::launch_prob_queries(st, d_queries, nq, pad, qs.fac_out, qs.eps_out, qs.norm_out, f8 ? nullptr : qs.operand_out, s));
     if (f8)
-        HIP_CHECK(vfsx::launch_f8_queries(d_queries, nq, st.dim, pad, (uint4 *)(base + w.operand), (uint32_t *)(base + w.q8_exp), raw, s));
+        HIP_CHECK(vfsx::launch_f8_queries(d_queries, nq, st.dim, pad, qs.operand_out, (uint32_t *)(base + w.q8_exp), raw, s));
+    return false;
 }
 
 void check_similarity(int similarity)
@@ -2158,10 +2168,11 @@ void log_probs_impl(vfsx_corpus *c, const LogProbsArgs &a, hipStream_t s, bool c
     for (uint32_t q0 = 0; q0 < a.nq; q0 += w.round) {
         const uint32_t qn = std::min(w.round, a.nq - q0);
         vfsx::ProbQueries qs{};
-        prepare_queries(st, w, base, a.queries + (size_t)q0 * c->dim, qn, f8, false, qs, s);
+        const bool few = prepare_queries(st, w, base, a.queries + (size_t)q0 * c->dim, qn, f8, false, qs, s);
         float4 *pieces = (float4 *)(base + w.pieces);
         float *groups = (float *)(base + w.groups);
-        HIP_CHECK(vfsx::launch_prob_pieces(st, qs, pieces, groups, s));
+        HIP_CHECK(few && st.n_pieces ? vfsx::launch_few_pieces(st, qs, pieces, groups, c->n_cus, s)
+                                     : vfsx::launch_prob_pieces(st, qs, pieces, groups, s));
         vfsx::ProbFinish f{};
         f.pieces = pieces;
         f.groups = groups;
@@ -2199,8 +2210,10 @@ void scores_f8_impl(vfsx_corpus *c, const float *d_queries, uint32_t nq, int sim
     for (uint32_t q0 = 0; q0 < nq; q0 += w.round) {
         const uint32_t qn = std::min(w.round, nq - q0);
         vfsx::ProbQueries qs{};
-        prepare_queries(st, w, c->prob_work.p, d_queries + (size_t)q0 * c->dim, qn, true, out_dtype == VFSX_SCORES_BF16, qs, s);
-        HIP_CHECK(vfsx::launch_f8_scores(st, qs, (char *)d_out + (size_t)q0 * ld * elem, ld, out_dtype == VFSX_SCORES_BF16, s));
+        const int bf16 = out_dtype == VFSX_SCORES_BF16;
+        const bool few = prepare_queries(st, w, c->prob_work.p, d_queries + (size_t)q0 * c->dim, qn, true, bf16 != 0, qs, s);
+        void *out = (char *)d_out + (size_t)q0 * ld * elem;
+        HIP_CHECK(few ? vfsx::launch_few_scores(st, qs, out, ld, bf16, c->n_cus, s) : vfsx::launch_f8_scores(st, qs, out, ld, bf16, s));
     }
 }
 

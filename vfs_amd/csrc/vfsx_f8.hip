@@ -18,25 +18,6 @@ namespace vfsx {
 
 namespace {
 
-// e of a block from the bits of max|x|: 448 = 1.75 * 2^8, so e = (exponent of max) - 8, one more when its leading digits pass 1.75
-__device__ __forceinline__ int f8_exponent(float top)
-{
-    const uint32_t b = __float_as_uint(top);
-    if (b == 0u || b >= 0x7f800000u)
-        return 0;
-    const int e = (int)(b >> 23) - 135 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
-    return e < -127 ? -127 : e;
-}
-
-// four values -> four e4m3 bytes; `by` = 2^-e (never subnormal: e <= 120)
-__device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d, float by)
-{
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * by, b * by, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * by, d * by, w, true);
-}
-
-__device__ __forceinline__ float pow2_neg(int e) { return __uint_as_float((uint32_t)(127 - e) << 23); }
-
 // One lane per row, one wave per (row-block, dword of four scales): reads the row's f32 chunks twice (maximum, then the values;
 // the second read comes from the cache), writes 16-byte chunks back to back over the 64 lanes.  Bound by reading the store
 // once; runs when rows were added.

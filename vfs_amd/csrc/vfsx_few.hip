@@ -1,0 +1,404 @@
+// vfsx_few.hip -- the first pass for up to 8 queries: the same products and statistics as vfsx_stream.hip, bound by reading the store.
+//
+// The operands change places: the queries are the matrix instruction's A (32 matrix rows, of which 1 to 8 are queries), the store's
+// rows its B, so that a lane ends with the products of ITS row and the queries in its first registers: the epilogue costs what the
+// queries there are cost, not 32 of them.  Nothing is shared between waves but the queries, which every workgroup prepares for itself in LDS
+// once (a launch less, and no barrier after that); each wave then walks its row-blocks, PF K-steps of loads ahead, across the
+// row-blocks' borders.
+//
+// int8 rows need no conversion here: a query is rounded to 23 bits and cut into three signed 8-bit digits, q = 2^-e (65536 d0 + 256 d1 + d2), which
+// take three of its eight matrix rows' places, and v_mfma_i32_32x32x32_i8 gives three exact integer products (2^-23 of the
+// largest element is lost, within the bound of vfsx_prob.hip).
+#include <hip/hip_runtime.h>
+
+#include "vfsx_device.h"
+#include "vfsx_internal.h"
+#include "vfsx_prob.h"
+#include "vfsx_prob_device.h"
+
+#pragma clang fp contract(off)
+
+namespace vfsx {
+
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+constexpr uint32_t kFewWaves = 4;
+
+// bytes that one element of one query takes in LDS
+template <int SRC>
+constexpr uint32_t kQueryBytes = SRC == kProbF32 ? 4u : (SRC == kProbI8 ? 3u : 2u);
+// a K-step: 8 loads of 16 bytes per lane (8 chunks of 64 rows)
+template <int SRC>
+constexpr uint32_t kStepElems = SRC == kProbF32 ? 32u : 128u;
+
+template <int J>
+__device__ __forceinline__ float xor_f(float v)
+{
+    return __uint_as_float(xor_lane32<J>(__float_as_uint(v)));
+}
+__device__ __forceinline__ float max8(float v) // over 8 neighbouring lanes
+{
+    v = fmaxf(v, xor_f<1>(v));
+    v = fmaxf(v, xor_f<2>(v));
+    return fmaxf(v, xor_f<4>(v));
+}
+template <bool ALL> // over 64 lanes (ALL) or the 32 of a half
+__device__ __forceinline__ float sum_lanes(float v)
+{
+    v += xor_f<1>(v);
+    v += xor_f<2>(v);
+    v += xor_f<4>(v);
+    v += xor_f<8>(v);
+    v += xor_f<16>(v);
+    if (ALL)
+        v += xor_f<32>(v);
+    return v;
+}
+
+// One wave: query qi of `src` (nullptr: none, zeros) -> its place `slot` of NQS in LDS; factor, whether it has no cosine.
+template <int SRC, uint32_t NQS>
+__device__ void prepare_query(const ProbStore &st, const float *src, uint32_t slot, uint32_t elems, uint8_t *lds, QueryFactors &out)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    double s = 0.0;
+    float top = 0.0f;
+    bool bad = false;
+    if (src) {
+        for (uint32_t j = lane; j < st.dim; j += 64u) {
+            const float v = src[j];
+            s = __builtin_fma((double)v, (double)v, s);
+            top = fmaxf(top, fabsf(v));
+            bad = bad || !(fabsf(v) < __builtin_inff());
+        }
+        for (int o = 32; o; o >>= 1) {
+            s += __shfl_xor(s, o, 64);
+            top = fmaxf(top, __shfl_xor(top, o, 64));
+        }
+        bad = __any(bad);
+    }
+    double scale = 1.0;
+    if constexpr (SRC == kProbF32) {
+        const float by = pair_scale(__builtin_sqrt(s));
+        scale = by;
+        for (uint32_t k = lane; k < elems; k += 64u) {
+            const float x = src && k < st.dim ? src[k] * by : 0.0f;
+            const _Float16 hi = (_Float16)x, lo = (_Float16)(x - (float)hi);
+            // piece (chunk of 8, part, query), 16 bytes each
+            uint8_t *at = lds + (((size_t)(k / 8u) * 2u) * NQS + slot) * 16u + (k & 7u) * 2u;
+            *(_Float16 *)at = hi;
+            *(_Float16 *)(at + NQS * 16u) = lo;
+        }
+    } else if constexpr (SRC == kProbI8) {
+        int e = 0;
+        if (top > 0.0f && !bad)
+            (void)frexp((double)top, &e); // top < 2^e
+        e = 22 - e;                       // |q| 2^e <= 2^22: the first digit stays within +-65
+        scale = bad ? __builtin_nan("") : ldexp(1.0, e);
+        for (uint32_t k = lane; k < elems; k += 64u) {
+            const int t = src && !bad && k < st.dim ? (int)rint(ldexp((double)src[k], e)) : 0;
+            const int d2 = (int8_t)t, r = (t - d2) >> 8, d1 = (int8_t)r, d0 = (r - d1) >> 8;
+            uint8_t *at = lds + (((size_t)(k / 16u) * 3u) * NQS + slot) * 16u + (k & 15u); // (chunk of 16, digit, query)
+            at[0] = (uint8_t)d0;
+            at[NQS * 16u] = (uint8_t)d1;
+            at[2u * NQS * 16u] = (uint8_t)d2;
+        }
+    } else {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        for (uint32_t k = 2u * lane; k < elems; k += kF8Block) { // a block of 128 at a time
+            const float a = src && k < st.dim ? src[k] : 0.0f, b = src && k + 1u < st.dim ? src[k + 1u] : 0.0f;
+            float m = fmaxf(fabsf(a), fabsf(b));
+            const bool nan = __any(!(fabsf(a) < __builtin_inff()) || !(fabsf(b) < __builtin_inff()));
+            for (int o = 32; o; o >>= 1)
+                m = fmaxf(m, __shfl_xor(m, o, 64));
+            const int e = nan ? 0 : f8_exponent(m);
+            const float by = pow2_neg(e);
+            const uint32_t w = nan ? 0x7f7fu : (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a * by, b * by, 0, false) & 0xffffu;
+            const bf16x2 v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, __uint_as_float((uint32_t)(e + 127) << 23), false);
+            *(uint32_t *)(lds + ((size_t)(k / 8u) * NQS + slot) * 16u + (k & 7u) * 2u) = __builtin_bit_cast(uint32_t, v);
+        }
+    }
+    out = query_factors(st, s, scale);
+}
+
+template <int SRC, uint32_t NQS, int EPI, uint32_t PF>
+__global__ __launch_bounds__(kFewWaves * 64, 3) void few_kernel(ProbStore st, const float *__restrict__ q, uint32_t nq, ProbQueries qs,
+                                                               StreamOut out, uint32_t elems)
+{
+    extern __shared__ __align__(16) uint8_t q_lds[]; // elems * NQS * kQueryBytes
+    __shared__ QueryFactors factors[NQS];
+    const uint32_t lane = threadIdx.x & 63u, h = lane >> 5, r32 = lane & 31u;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    for (uint32_t i = wave; i < NQS; i += kFewWaves) {
+        QueryFactors f;
+        prepare_query<SRC, NQS>(st, i < nq ? q + (size_t)i * st.dim : nullptr, i, elems, q_lds, f);
+        if (lane == 0) {
+            factors[i] = f;
+            if (blockIdx.x == 0 && i < nq) { // for the second pass
+                qs.fac_out[i] = f.fac;
+                qs.eps_out[i] = f.eps;
+                qs.norm_out[i] = f.norm;
+            }
+        }
+    }
+    __syncthreads();
+    if (SRC == kProbF8 && blockIdx.x == 0)
+        for (uint32_t i = threadIdx.x; i < elems / 8u * NQS; i += kFewWaves * 64u)
+            qs.operand_out[i] = ((const uint4 *)q_lds)[i];
+
+    const uint32_t n_rb = (st.n_rows + 63u) / 64u, n_step = (st.dim + kStepElems<SRC> - 1u) / kStepElems<SRC>;
+    const uint32_t first = blockIdx.x * kFewWaves + wave, stride = gridDim.x * kFewWaves;
+    if (first >= n_rb)
+        return;
+    const uint32_t my_rb = (n_rb - first + stride - 1u) / stride, total = my_rb * n_step;
+    const uint32_t row_chunks = SRC == kProbF8 ? st.f8_chunks : st.d_chunks;
+    const uint4 *rows = SRC == kProbF8 ? st.f8 : st.rows;
+
+    // ---- loads, PF K-steps ahead -----------------------------------------------------------------------------------------------------
+    struct Ahead {
+        u32x4 a[8];
+        uint32_t of_row[2]; // f32: the rows' scales; f8: their dwords of exponents
+    };
+    Ahead ahead[PF];
+    uint32_t p_rb = first, p_step = 0;
+    auto load = [&](Ahead &x) {
+        // bounded by the row-block: chunks beyond a row's last read as zeros
+        const __amdgpu_buffer_rsrc_t rsrc =
+            __builtin_amdgcn_make_buffer_rsrc((void *)(rows + (size_t)p_rb * row_chunks * 64u), 0, row_chunks * 1024u, 0x00020000);
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) {
+            const uint32_t tile = i >> 2, j = i & 3u;
+            const uint32_t c = SRC == kProbF32 ? 4u * (j >> 1) + 2u * h + (j & 1u) : 2u * j + h;
+            x.a[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)((p_step * 8u + c) * 1024u + (tile * 32u + r32) * 16u), 0, 2 /* streamed */);
+        }
+#pragma unroll
+        for (uint32_t tile = 0; tile < 2u; ++tile) {
+            if (SRC == kProbF32)
+                x.of_row[tile] = __float_as_uint(st.row_scale[p_rb * 64u + tile * 32u + r32]);
+            if (SRC == kProbF8)
+                x.of_row[tile] = st.f8_exp[((size_t)p_rb * st.f8_words + (p_step >> 2)) * 64u + tile * 32u + r32];
+        }
+        if (++p_step == n_step) {
+            p_step = 0;
+            p_rb = p_rb + stride < n_rb ? p_rb + stride : p_rb; // (past the end: the last one again)
+        }
+    };
+#pragma unroll
+    for (uint32_t p = 0; p < PF; ++p)
+        load(ahead[p]);
+
+    // ---- epilogue of a row-block -------------------------------------------------------------------------------------------------------
+    using Acc = typename std::conditional<SRC == kProbI8, i32x16, f32x16>::type;
+    Acc acc[2] = {};
+    constexpr uint32_t SLOTS = NQS < 4u ? NQS : 4u;
+    // NQS <= 4: both halves of the wave hold the same products; half h goes on with tile h, one row per lane.  NQS = 8: half h holds queries
+    // 4 h .. 4 h + 3 and both tiles.
+    constexpr uint32_t TILES = NQS <= 4u ? 1u : 2u;
+    auto product = [&](uint32_t tile, uint32_t b) -> float {
+        if constexpr (SRC == kProbI8)
+            return __builtin_fmaf((float)acc[tile][b], 65536.0f, __builtin_fmaf((float)acc[tile][4u + b], 256.0f, (float)acc[tile][8u + b]));
+        else
+            return acc[tile][b];
+    };
+    auto finish_block = [&](uint32_t rb) __attribute__((always_inline)) {
+        float mul[TILES], add[TILES];
+        bool gone[TILES];
+#pragma unroll
+        for (uint32_t t = 0; t < TILES; ++t) {
+            const uint32_t row = rb * 64u + (TILES == 1u ? lane : t * 32u + r32);
+            gone[t] = row >= st.n_rows;
+            add[t] = 0.0f;
+            mul[t] = 1.0f;
+            if (!gone[t]) {
+                if (EPI == kPieces && st.bias)
+                    add[t] = st.bias[row];
+                if (st.cosine)
+                    mul[t] = st.row_inv[row];
+                gone[t] = EPI == kPieces && (add[t] == neg_inf() || (st.cosine && mul[t] < 0.0f));
+                if (EPI != kPieces && st.cosine && mul[t] < 0.0f)
+                    mul[t] = __builtin_nanf("");
+                if (SRC == kProbF32) // / 2^a
+                    mul[t] *= __uint_as_float((254u << 23) - __float_as_uint(st.row_scale[row]));
+            }
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < SLOTS; ++b) {
+            const uint32_t qi = NQS <= 4u ? b : 4u * h + b;
+            if (NQS <= 4u && b >= nq)
+                break;
+            const QueryFactors f = factors[qi];
+            float l[TILES];
+#pragma unroll
+            for (uint32_t t = 0; t < TILES; ++t)
+                l[t] = TILES == 1u ? (h ? product(1, b) : product(0, b)) : product(t, b);
+            if constexpr (EPI == kPieces) {
+                const bool q_gone = st.cosine && f.norm == 0.0;
+                float g[TILES], m = neg_inf(), s = 0.0f, u = 0.0f;
+#pragma unroll
+                for (uint32_t t = 0; t < TILES; ++t) {
+                    l[t] = gone[t] || q_gone ? neg_inf() : __builtin_fmaf(l[t], f.fac * mul[t], add[t]);
+                    g[t] = max8(l[t]);
+                    m = fmaxf(m, g[t]);
+                }
+                m = fmaxf(m, xor_f<8>(m));
+                m = fmaxf(m, xor_f<16>(m));
+                if (TILES == 1u)
+                    m = fmaxf(m, xor_f<32>(m));
+                const float base = piece_base(m);
+                const bool huge = piece_is_huge(m);
+#pragma unroll
+                for (uint32_t t = 0; t < TILES; ++t) {
+                    const float z = huge ? (l[t] - m) * kLog2e : __builtin_fmaf(l[t], kLog2e, -base);
+                    const float e = __builtin_amdgcn_exp2f(z);
+                    // (a row there whose logit is infinite spoils the sums; a very low finite one adds nothing)
+                    const bool out_of_it = gone[t] || q_gone;
+                    s += out_of_it ? 0.0f : (fabsf(l[t]) < __builtin_inff() ? e : __builtin_nanf(""));
+                    u += out_of_it || e == 0.0f ? 0.0f : e * z;
+                }
+                s = sum_lanes<TILES == 1u>(s);
+                u = sum_lanes<TILES == 1u>(u);
+                if (qi < nq) {
+                    const size_t piece = (size_t)qi * st.n_pieces + rb;
+                    if ((TILES == 1u ? lane : r32) == 0u)
+                        out.pieces[piece] = make_float4(m, s, u, 0.0f);
+#pragma unroll
+                    for (uint32_t t = 0; t < TILES; ++t)
+                        if ((lane & 7u) == 0u)
+                            out.groups[piece * kGroupsPerPiece + (TILES == 1u ? lane >> 3 : 4u * t + (r32 >> 3))] = g[t];
+                }
+            } else {
+                const float fac = st.cosine && f.norm == 0.0 ? __builtin_nanf("") : f.fac;
+#pragma unroll
+                for (uint32_t t = 0; t < TILES; ++t) {
+                    const uint32_t row = rb * 64u + (TILES == 1u ? lane : t * 32u + r32);
+                    const float v = l[t] * fac * mul[t];
+                    if (row < st.n_rows && qi < nq) {
+                        if (EPI == kScoresF32)
+                            ((float *)out.scores)[(size_t)qi * out.ld + row] = v;
+                        else
+                            ((__bf16 *)out.scores)[(size_t)qi * out.ld + row] = (__bf16)v;
+                    }
+                }
+            }
+        }
+    };
+
+    // ---- the walk ------------------------------------------------------------------------------------------------------------------------
+    const uint4 *q_at = (const uint4 *)q_lds;
+    const uint32_t my_q = r32 & (NQS - 1u) & 7u, my_digit = (r32 >> 3) == 3u ? 0u : r32 >> 3; // of matrix row r32
+    uint32_t rb = first, step = 0;
+    for (uint32_t i0 = 0; i0 < total; i0 += PF) {
+#pragma unroll
+        for (uint32_t p = 0; p < PF; ++p) {
+            if (i0 + p >= total)
+                break;
+            Ahead &x = ahead[p];
+            if constexpr (SRC == kProbI8) {
+#pragma unroll
+                for (uint32_t s = 0; s < 4u; ++s) { // 32 elements: chunks 2 s and 2 s + 1
+                    const i32x4 d = __builtin_bit_cast(i32x4, q_at[((step * 8u + 2u * s + h) * 3u + my_digit) * NQS + my_q]);
+#pragma unroll
+                    for (uint32_t t = 0; t < 2u; ++t)
+                        acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(d, __builtin_bit_cast(i32x4, x.a[4u * t + s]), acc[t], 0, 0, 0);
+                }
+            } else {
+                constexpr uint32_t kSlices = kStepElems<SRC> / 16u;
+#pragma unroll
+                for (uint32_t s = 0; s < kSlices; ++s) {
+                    const uint32_t qc = SRC == kProbF32 ? step * 4u + 2u * s + h : step * 16u + 4u * (s >> 1) + 2u * h + (s & 1u);
+                    u32x4 qh, ql;
+                    if constexpr (SRC == kProbF32) {
+                        qh = __builtin_bit_cast(u32x4, q_at[(qc * 2u) * NQS + my_q]);
+                        ql = __builtin_bit_cast(u32x4, q_at[(qc * 2u + 1u) * NQS + my_q]);
+                    } else {
+                        qh = ql = __builtin_bit_cast(u32x4, q_at[qc * NQS + my_q]);
+                    }
+#pragma unroll
+                    for (uint32_t t = 0; t < 2u; ++t) {
+                        if constexpr (SRC == kProbF32) {
+                            const u32x4 u = x.a[4u * t + 2u * s], v = x.a[4u * t + 2u * s + 1u];
+                            const float by = __uint_as_float(x.of_row[t]);
+                            float e[8];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                e[i] = __uint_as_float(u[i]) * by;
+                                e[i + 4] = __uint_as_float(v[i]) * by;
+                            }
+                            const HalfPair r = split8(e);
+                            acc[t] = mfma16<SRC>(ql, __builtin_bit_cast(u32x4, r.hi), acc[t]);
+                            acc[t] = mfma16<SRC>(qh, __builtin_bit_cast(u32x4, r.lo), acc[t]);
+                            acc[t] = mfma16<SRC>(qh, __builtin_bit_cast(u32x4, r.hi), acc[t]);
+                        } else {
+                            const u32x4 u = x.a[4u * t + (s >> 1)];
+                            const float by = __uint_as_float(((x.of_row[t] >> (8u * (step & 3u))) & 255u) << 23);
+                            acc[t] = mfma16<SRC>(qh, bf16_of_e4m3(u[(s & 1u) * 2u], u[(s & 1u) * 2u + 1u], by), acc[t]);
+                        }
+                    }
+                }
+            }
+            load(x);
+            if (++step == n_step) {
+                finish_block(rb);
+                acc[0] = Acc{};
+                acc[1] = Acc{};
+                step = 0;
+                rb += stride;
+            }
+        }
+    }
+}
+
+template <int SRC, uint32_t NQS, int EPI>
+hipError_t few(const ProbStore &st, const ProbQueries &qs, const StreamOut &out, uint32_t n_cus, hipStream_t s)
+{
+    constexpr uint32_t PF = 2;
+    const uint32_t elems = query_elems(st.dim), n_rb = (st.n_rows + 63u) / 64u;
+    const size_t lds = (size_t)elems * NQS * kQueryBytes<SRC>;
+    // as many workgroups as stay resident (three by registers, fewer by LDS), in even shares
+    const uint32_t per_cu = lds > 48u * 1024u ? 2u : 3u;
+    const uint32_t tiles = (n_rb + kFewWaves - 1u) / kFewWaves;
+    uint32_t grid = tiles < n_cus * per_cu ? tiles : n_cus * per_cu;
+    const uint32_t rounds = (tiles + grid - 1u) / grid;
+    grid = (tiles + rounds - 1u) / rounds;
+    few_kernel<SRC, NQS, EPI, PF><<<grid, kFewWaves * 64u, lds, s>>>(st, qs.q, qs.nq, qs, out, elems);
+    return hipGetLastError();
+}
+
+template <int SRC, int EPI>
+hipError_t few_for(const ProbStore &st, const ProbQueries &qs, const StreamOut &out, uint32_t n_cus, hipStream_t s)
+{
+    switch (few_places(qs.nq)) {
+    case 1:
+        return few<SRC, 1, EPI>(st, qs, out, n_cus, s);
+    case 2:
+        return few<SRC, 2, EPI>(st, qs, out, n_cus, s);
+    case 4:
+        return few<SRC, 4, EPI>(st, qs, out, n_cus, s);
+    default:
+        return few<SRC, 8, EPI>(st, qs, out, n_cus, s);
+    }
+}
+
+} // namespace
+
+hipError_t launch_few_pieces(const ProbStore &st, const ProbQueries &q, float4 *pieces, float *groups, uint32_t n_cus, hipStream_t s)
+{
+    if (!st.n_pieces)
+        return hipSuccess;
+    const StreamOut out{pieces, groups, nullptr, 0, 0};
+    if (st.source == kProbI8)
+        return few_for<kProbI8, kPieces>(st, q, out, n_cus, s);
+    if (st.source == kProbF8)
+        return few_for<kProbF8, kPieces>(st, q, out, n_cus, s);
+    return few_for<kProbF32, kPieces>(st, q, out, n_cus, s);
+}
+
+hipError_t launch_few_scores(const ProbStore &st, const ProbQueries &q, void *scores, uint64_t ld, int bf16, uint32_t n_cus, hipStream_t s)
+{
+    const StreamOut out{nullptr, nullptr, scores, ld, 0};
+    return bf16 ? few_for<kProbF8, kScoresBf16>(st, q, out, n_cus, s) : few_for<kProbF8, kScoresF32>(st, q, out, n_cus, s);
+}
+
+} // namespace vfsx

@@ -27,6 +27,10 @@ constexpr uint32_t kGroupsPerPiece = kPieceRows / kGroupRows;
 
 enum ProbSource { kProbF32 = 0, kProbI8 = 1, kProbF8 = 2 };
 
+// elements of one query operand: whole blocks, which are whole K-steps of every kind
+constexpr uint32_t kQueryPad = 128;
+inline uint32_t query_elems(uint32_t dim) { return (dim + kQueryPad - 1u) / kQueryPad * kQueryPad; }
+
 // what a pass over the store reads; the same for every query
 struct ProbStore {
     int source;            // ProbSource
@@ -52,6 +56,11 @@ struct ProbQueries {
     const float *eps;      // [nq] how far a first-pass logit may be from its value, relative to its row's part (see vfsx_prob.hip)
     const double *norm;    // [nq] |q|; 0: the query has no cosine
     uint32_t nq;
+    uint32_t operand_chunk; // bf16 operand: distance of a query's chunks (64, or the places of launch_few_pieces)
+    // the same arrays, where the first pass itself prepares the queries (launch_few_*)
+    float *fac_out, *eps_out;
+    double *norm_out;
+    uint4 *operand_out;
 };
 
 // pieces of a long store, joined by 64: sums over 2^(l log2e - base of m)
@@ -77,10 +86,6 @@ struct ProbFinish {
     uint32_t n_units;
 };
 
-// elements of one query operand: whole blocks, which are whole K-steps of every kind
-constexpr uint32_t kQueryPad = 128;
-inline uint32_t query_elems(uint32_t dim) { return (dim + kQueryPad - 1u) / kQueryPad * kQueryPad; }
-
 hipError_t launch_prob_rows(const ProbStore &st, uint32_t row0, float *row_inv, float *row_scale, float *max_norm, hipStream_t s);
 // nq_pad: whole tiles of queries; those beyond nq become zeros.  `pairs` nullptr: only the factors (source f8)
 hipError_t launch_prob_queries(const ProbStore &st, const float *q, uint32_t nq, uint32_t nq_pad, float *fac, float *eps, double *norm,
@@ -98,6 +103,18 @@ inline uint32_t stream_query_pad(uint32_t nq)
 hipError_t launch_prob_pieces(const ProbStore &st, const ProbQueries &q, float4 *pieces, float *groups, hipStream_t s);
 // out[nq][ld]: f32 (bf16 = 0) or bf16
 hipError_t launch_f8_scores(const ProbStore &st, const ProbQueries &q, void *out, uint64_t ld, int bf16, hipStream_t s);
+
+// vfsx_few.hip: the first pass for up to 8 queries; prepares them itself
+constexpr uint32_t kFewQueries = 8;
+constexpr uint32_t kFewLdsBytes = 64u << 10; // of queries
+inline uint32_t few_places(uint32_t nq) { return nq <= 2u ? nq : (nq <= 4u ? 4u : 8u); }
+inline bool few_takes(uint32_t nq, uint32_t dim, int source)
+{
+    const uint64_t bytes = source == kProbF32 ? 4u : (source == kProbI8 ? 3u : 2u);
+    return nq <= kFewQueries && bytes * query_elems(dim) * few_places(nq) <= kFewLdsBytes;
+}
+hipError_t launch_few_pieces(const ProbStore &st, const ProbQueries &q, float4 *pieces, float *groups, uint32_t n_cus, hipStream_t s);
+hipError_t launch_few_scores(const ProbStore &st, const ProbQueries &q, void *out, uint64_t ld, int bf16, uint32_t n_cus, hipStream_t s);
 
 // vfsx_f8.hip
 hipError_t launch_f8_rows(const uint4 *rows, uint32_t d_chunks, uint32_t dim, uint32_t row0, uint32_t n_rows, uint32_t n_pad,

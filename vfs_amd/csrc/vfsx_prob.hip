@@ -31,21 +31,6 @@ namespace vfsx {
 
 namespace {
 
-// 2^a, the scale that brings vectors of norm r into the range of f16 pairs: r 2^a in (2^9, 2^10], so that elements 2^19 times smaller
-// than the norm still have a normal low half.  r = 0: 1; NaN or infinite: NaN.
-__device__ __forceinline__ float pair_scale(double r)
-{
-    if (!(r < __builtin_inf()))
-        return __builtin_nanf("");
-    if (r == 0.0)
-        return 1.0f;
-    int e;
-    (void)frexp(r, &e); // r = m 2^e, m in [0.5, 1)
-    e = 10 - e;
-    e = e > 126 ? 126 : (e < -126 ? -126 : e);
-    return __uint_as_float((uint32_t)(127 + e) << 23);
-}
-
 // ---- operands of a store: 1 / |x| per row, the largest |x| -------------------------------------------------------------------
 // One thread per row.  Norms in f64: they divide every logit.  A norm whose square is zero in f32 counts as zero.
 template <int SRC>
@@ -115,14 +100,10 @@ __global__ __launch_bounds__(64) void prob_queries_kernel(ProbStore st, const fl
     }
     if (lane || !there)
         return;
-    const bool zero = (float)s == 0.0f;
-    norm[qi] = zero ? 0.0 : r;
-    const double by = (pairs ? (double)scale : 1.0) * st.divide;
-    fac[qi] = (float)(1.0 / (st.cosine ? (zero ? by : by * r) : by));
-    const double part = st.cosine ? 1.0 : r * (double)*st.max_norm;
-    // 8-bit copies are up to 1 + 2^-4 times as long as their originals, each
-    const double e = (double)(st.dim + 64u) * 0x1p-24 * (st.source == kProbF8 ? 1.25 : 1.0) * part / __builtin_fabs(st.divide);
-    eps[qi] = (float)(e * (1.0 + 0x1p-20));
+    const QueryFactors f = query_factors(st, s, pairs ? (double)scale : 1.0);
+    norm[qi] = f.norm;
+    fac[qi] = f.fac;
+    eps[qi] = f.eps;
 }
 
 // ---- second pass -----------------------------------------------------------------------------------------------------------------
@@ -153,11 +134,12 @@ __device__ __forceinline__ T row_dot(const ProbStore &st, const ProbQueries &qs,
     T dot = 0;
     if constexpr (SRC == kProbF8) {
         const uint4 *x = st.f8 + (size_t)(row / 64u) * st.f8_chunks * 64u + (row & 63u);
-        const uint4 *q = qs.operand + (size_t)(qi / 64u) * st.f8_chunks * 128u + (qi & 63u);
+        const uint32_t qc = qs.operand_chunk; // (a query's chunks: this far apart; blocks of 64 queries)
+        const uint4 *q = qs.operand + (size_t)(qi / 64u) * st.f8_chunks * 2u * qc + (qi & 63u);
         const uint32_t *xe = st.f8_exp + (size_t)(row / 64u) * st.f8_words * 64u + (row & 63u);
 #pragma unroll 4
         for (uint32_t c = first; c < st.f8_chunks; c += step)
-            dot += scaled(f8_chunk_dot<T>(x[(size_t)c * 64u], q[(size_t)c * 128u], q[(size_t)c * 128u + 64u]), f8_exp_of(xe, c / kF8ChunksPerBlock));
+            dot += scaled(f8_chunk_dot<T>(x[(size_t)c * 64u], q[(size_t)c * 2u * qc], q[((size_t)c * 2u + 1u) * qc]), f8_exp_of(xe, c / kF8ChunksPerBlock));
     }
     if constexpr (SRC != kProbF8 || SQ) {
         if (SRC != kProbF8 || st.cosine) {

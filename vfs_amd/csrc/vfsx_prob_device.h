@@ -3,10 +3,29 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "vfsx_prob.h"
 
 namespace vfsx {
 namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+enum Epilogue { kPieces = 0, kScoresF32 = 1, kScoresBf16 = 2 };
+
+struct StreamOut {
+    float4 *pieces;
+    float *groups;
+    void *scores;
+    uint64_t ld;
+    int aligned; // every run of 16 scores starts at a multiple of 16 bytes
+};
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
@@ -103,6 +122,113 @@ __device__ __forceinline__ float piece_base(float m) { return m * kLog2e; }
 __device__ __forceinline__ bool piece_is_huge(float m) { return !(fabsf(m) < 1e30f); }
 // ... in f64, in units of log 2
 __device__ __forceinline__ double piece_base64(float m) { return piece_is_huge(m) ? (double)m * (double)kLog2e : (double)piece_base(m); }
+
+struct HalfPair {
+    f16x8 hi, lo;
+};
+
+__device__ __forceinline__ HalfPair split8(const float *x)
+{
+    HalfPair r;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const f32x2 v = {x[i], x[i + 1]};
+        const f16x2 h = __builtin_convertvector(v, f16x2);
+        const f32x2 rest = {__builtin_fmaf((float)h[0], -1.0f, x[i]), __builtin_fmaf((float)h[1], -1.0f, x[i + 1])};
+        const f16x2 l = __builtin_convertvector(rest, f16x2);
+        r.hi[i] = h[0], r.hi[i + 1] = h[1];
+        r.lo[i] = l[0], r.lo[i + 1] = l[1];
+    }
+    return r;
+}
+
+__device__ __forceinline__ f16x8 halves8(uint32_t a, uint32_t b) // 8 int8 values
+{
+    f16x8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r[i] = (_Float16)i8_at(a, i);
+        r[i + 4] = (_Float16)i8_at(b, i);
+    }
+    return r;
+}
+
+// 8 e4m3 values times a power of two (the exponent of `scale`, which is an e8m0 byte in its place): exact in bf16
+__device__ __forceinline__ u32x4 bf16_of_e4m3(uint32_t a, uint32_t b, float scale)
+{
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true),
+                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, true)};
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r[i] = __builtin_bit_cast(uint32_t, v[i]);
+    return r;
+}
+
+template <int SRC>
+__device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c)
+{
+    typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+    if constexpr (SRC == kProbF8)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// e of a block from the bits of max|x|: 448 = 1.75 * 2^8, so e = (exponent of max) - 8, one more when its leading digits pass 1.75
+__device__ __forceinline__ int f8_exponent(float top)
+{
+    const uint32_t b = __float_as_uint(top);
+    if (b == 0u || b >= 0x7f800000u)
+        return 0;
+    const int e = (int)(b >> 23) - 135 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < -127 ? -127 : e;
+}
+
+// four values -> four e4m3 bytes; `by` = 2^-e (never subnormal: e <= 120)
+__device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d, float by)
+{
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * by, b * by, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * by, d * by, w, true);
+}
+
+__device__ __forceinline__ float pow2_neg(int e) { return __uint_as_float((uint32_t)(127 - e) << 23); }
+
+// 2^a, the scale that brings vectors of norm r into the range of f16 pairs: r 2^a in (2^9, 2^10], so that elements 2^19 times smaller
+// than the norm still have a normal low half.  r = 0: 1; NaN or infinite: NaN.
+__device__ __forceinline__ float pair_scale(double r)
+{
+    if (!(r < __builtin_inf()))
+        return __builtin_nanf("");
+    if (r == 0.0)
+        return 1.0f;
+    int e;
+    (void)frexp(r, &e); // r = m 2^e, m in [0.5, 1)
+    e = 10 - e;
+    e = e > 126 ? 126 : (e < -126 ? -126 : e);
+    return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
+// What a query's products are multiplied by, and how far they may be off, from its sum of squares; `scale`: what its operand is scaled by.
+struct QueryFactors {
+    double norm; // 0: no cosine
+    float fac;   // logit = product * fac [/ |x|] + bias
+    float eps;
+};
+__device__ __forceinline__ QueryFactors query_factors(const ProbStore &st, double sum_sq, double scale)
+{
+    QueryFactors r;
+    const double norm = __builtin_sqrt(sum_sq), by = scale * st.divide;
+    const bool zero = (float)sum_sq == 0.0f;
+    r.norm = zero ? 0.0 : norm;
+    r.fac = (float)(1.0 / (st.cosine && !zero ? by * norm : by));
+    const double part = st.cosine ? 1.0 : norm * (double)*st.max_norm;
+    // 8-bit copies are up to 1 + 2^-4 times as long as their originals, each
+    const double e = (double)(st.dim + 64u) * 0x1p-24 * (st.source == kProbF8 ? 1.25 : 1.0) * part / __builtin_fabs(st.divide);
+    r.eps = (float)(e * (1.0 + 0x1p-20));
+    return r;
+}
 
 // adds sums (s, u) over the base of m_part to sums over the base of m; s = 0: nothing there, NaN: a logit that is not finite
 __device__ __forceinline__ void add_unit(float m, float m_part, double s, double u, double &S, double &U)

@@ -32,24 +32,7 @@ namespace vfsx {
 
 namespace {
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
 enum { kF8Raw = 3 }; // beside ProbSource
-enum Epilogue { kPieces = 0, kScoresF32 = 1, kScoresBf16 = 2 };
-
-struct StreamOut {
-    float4 *pieces;
-    float *groups;
-    void *scores;
-    uint64_t ld;
-    int aligned; // every run of 16 scores starts at a multiple of 16 bytes
-};
-
 // What one K-step is.  Rows: kLoads loads of 16 bytes per lane (two tiles, each lane half every other chunk).  Queries: kQChunks chunks of
 // 16 bytes in kQParts parts (hi, lo), three slots of which leave room for two workgroups per CU.
 template <int SRC, int NT>
@@ -61,59 +44,6 @@ struct Step {
     static constexpr uint32_t kQParts = SRC == kProbF32 || SRC == kProbI8 ? 2u : 1u;
     static constexpr uint32_t kSlotBytes = kQChunks * kQParts * NT * 512u;
 };
-
-struct HalfPair {
-    f16x8 hi, lo;
-};
-
-__device__ __forceinline__ HalfPair split8(const float *x)
-{
-    HalfPair r;
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const f32x2 v = {x[i], x[i + 1]};
-        const f16x2 h = __builtin_convertvector(v, f16x2);
-        const f32x2 rest = {__builtin_fmaf((float)h[0], -1.0f, x[i]), __builtin_fmaf((float)h[1], -1.0f, x[i + 1])};
-        const f16x2 l = __builtin_convertvector(rest, f16x2);
-        r.hi[i] = h[0], r.hi[i + 1] = h[1];
-        r.lo[i] = l[0], r.lo[i + 1] = l[1];
-    }
-    return r;
-}
-
-__device__ __forceinline__ f16x8 halves8(uint32_t a, uint32_t b) // 8 int8 values
-{
-    f16x8 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        r[i] = (_Float16)i8_at(a, i);
-        r[i + 4] = (_Float16)i8_at(b, i);
-    }
-    return r;
-}
-
-// 8 e4m3 values times a power of two (the exponent of `scale`, which is an e8m0 byte in its place): exact in bf16
-__device__ __forceinline__ u32x4 bf16_of_e4m3(uint32_t a, uint32_t b, float scale)
-{
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    const bf16x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true),
-                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false), __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, true)};
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        r[i] = __builtin_bit_cast(uint32_t, v[i]);
-    return r;
-}
-
-template <int SRC>
-__device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c)
-{
-    typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-    if constexpr (SRC == kProbF8)
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
 
 template <int SRC, int NT, int WAVES, int EPI>
 __global__ __launch_bounds__(WAVES * 64, NT == 4 ? 2 : (NT == 2 ? 3 : 4)) void stream_kernel(ProbStore st, ProbQueries qs, StreamOut out, uint32_t n_rowtiles,
