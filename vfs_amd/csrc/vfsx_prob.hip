@@ -21,6 +21,7 @@
 // A logit that is NaN or infinite makes s or t NaN (inf - inf, 0 * inf), and with it every result of its query.
 #include <hip/hip_runtime.h>
 
+#include "vfsx_device.h"
 #include "vfsx_internal.h"
 #include "vfsx_prob.h"
 #include "vfsx_prob_device.h"
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(64) void prob_queries_kernel(ProbStore st, const fl
 // by what the candidate groups read for a batch: k groups or a few more, each 8 rows = 128 bytes, one cache line, of every chunk.
 constexpr uint32_t kFinGroups = 1024; // candidate groups kept at once
 constexpr uint32_t kFinRows = 1024;   // candidate rows kept at once
-constexpr uint32_t kBuckets = 256;    // maxima that the first bound is taken from; >= VFSX_LOG_PROBS_MAX_K
+constexpr uint32_t kBuckets = 256;    // maxima that the first bound of many rows is taken from
 static_assert(kBuckets >= VFSX_LOG_PROBS_MAX_K, "the first bound is one of them");
 
 struct FinCand {
@@ -121,13 +122,55 @@ struct FinCand {
     uint32_t pad;
 };
 
+template <int J>
+__device__ __forceinline__ double xor_d(double v)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, ((uint64_t)xor_lane32<J>((uint32_t)(b >> 32)) << 32) | xor_lane32<J>((uint32_t)b));
+}
+__device__ __forceinline__ double wave_sum(double v)
+{
+    v += xor_d<1>(v);
+    v += xor_d<2>(v);
+    v += xor_d<4>(v);
+    v += xor_d<8>(v);
+    v += xor_d<16>(v);
+    return v + xor_d<32>(v);
+}
+__device__ __forceinline__ float wave_max(float v)
+{
+    v = fmaxf(v, __uint_as_float(xor_lane32<1>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(xor_lane32<2>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(xor_lane32<4>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(xor_lane32<8>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(xor_lane32<16>(__float_as_uint(v))));
+    return fmaxf(v, __uint_as_float(xor_lane32<32>(__float_as_uint(v))));
+}
+__device__ __forceinline__ double lane_d(double v, uint32_t l)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), (int)l) << 32) |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)b, (int)l));
+}
+// the k-th largest of 64 values (1 <= k <= 64), by one wave; `lds`: the same values.  It is the smallest value that fewer than k are above.
+__device__ __forceinline__ float wave_kth(float v, const float *lds, uint32_t k)
+{
+    uint32_t above = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 64u; j += 4u) {
+        const float4 o = *(const float4 *)(lds + j);
+        above += (o.x > v ? 1u : 0u) + (o.y > v ? 1u : 0u) + (o.z > v ? 1u : 0u) + (o.w > v ? 1u : 0u);
+    }
+    return -wave_max(above < k ? -v : neg_inf());
+}
+
 __device__ __forceinline__ bool row_is_there(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row)
 {
     return row < st.n_rows && !(st.bias && st.bias[row] == neg_inf()) && !(st.cosine && (!(st.row_inv[row] >= 0.0f) || qs.norm[qi] == 0.0));
 }
 
 // q . x over chunks first, first + step, ... of one row, in f32 or f64; sq: the sum of squares too (f64, cosine)
-template <int SRC, typename T, bool SQ>
+template <int SRC, typename T, bool SQ, int UNROLL>
 __device__ __forceinline__ T row_dot(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row, uint32_t first, uint32_t step,
                                      double &sq)
 {
@@ -137,7 +180,7 @@ __device__ __forceinline__ T row_dot(const ProbStore &st, const ProbQueries &qs,
         const uint32_t qc = qs.operand_chunk; // (a query's chunks: this far apart; blocks of 64 queries)
         const uint4 *q = qs.operand + (size_t)(qi / 64u) * st.f8_chunks * 2u * qc + (qi & 63u);
         const uint32_t *xe = st.f8_exp + (size_t)(row / 64u) * st.f8_words * 64u + (row & 63u);
-#pragma unroll 4
+#pragma unroll UNROLL
         for (uint32_t c = first; c < st.f8_chunks; c += step)
             dot += scaled(f8_chunk_dot<T>(x[(size_t)c * 64u], q[(size_t)c * 2u * qc], q[((size_t)c * 2u + 1u) * qc]), f8_exp_of(xe, c / kF8ChunksPerBlock));
     }
@@ -147,7 +190,7 @@ __device__ __forceinline__ T row_dot(const ProbStore &st, const ProbQueries &qs,
             const float *q = qs.q + (size_t)qi * st.dim;
             constexpr uint32_t per = SRC == kProbI8 ? 16u : 4u;
             const uint32_t full = st.dim / per; // chunks without padding
-#pragma unroll 4
+#pragma unroll UNROLL
             for (uint32_t c = first; c < full; c += step) {
                 const uint4 v = p[(size_t)c * 64u];
                 if constexpr (SRC != kProbF8)
@@ -167,36 +210,41 @@ __device__ __forceinline__ T row_dot(const ProbStore &st, const ProbQueries &qs,
     return dot;
 }
 
+__device__ __forceinline__ double logit_of(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row, double dot, double sq)
+{
+    return (st.cosine ? dot / (qs.norm[qi] * __builtin_sqrt(sq) * st.divide) : dot / st.divide) + (double)(st.bias ? st.bias[row] : 0.0f);
+}
+
 // the logit of one row in f64, by a whole wave
 template <int SRC>
 __device__ __forceinline__ double row_logit(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row)
 {
     if (!row_is_there(st, qs, qi, row)) // (uniform)
         return -__builtin_inf();
-    double sq = 0.0, dot = row_dot<SRC, double, true>(st, qs, qi, row, threadIdx.x & 63u, 64u, sq);
-    for (int o = 1; o < 64; o <<= 1) {
-        dot += __shfl_xor(dot, o, 64);
-        if (st.cosine)
-            sq += __shfl_xor(sq, o, 64);
-    }
-    return (st.cosine ? dot / (qs.norm[qi] * __builtin_sqrt(sq) * st.divide) : dot / st.divide) + (double)(st.bias ? st.bias[row] : 0.0f);
+    double sq = 0.0, dot = row_dot<SRC, double, true, 4>(st, qs, qi, row, threadIdx.x & 63u, 64u, sq);
+    dot = wave_sum(dot);
+    if (st.cosine)
+        sq = wave_sum(sq);
+    return logit_of(st, qs, qi, row, dot, sq);
 }
 
-// the logits of a group's 8 rows in f32, row lane & 7 on every lane; eighths of a wave take every eighth chunk.  -inf: not there
-template <int SRC>
+// the logits of a group's 8 rows in f32 (as good as the first pass'), row lane & 7 on every lane; eighths of a wave take every eighth chunk.
+// -inf: not there.  (All of it in f64 instead, which saves the step after it: 15 us for 11 groups of 768 elements, this 4: two
+// conversions at a quarter rate for each product.)
+template <int SRC, int UNROLL>
 __device__ __forceinline__ float group_logit(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t group, float fac)
 {
     const uint32_t lane = threadIdx.x & 63u, row = group * kGroupRows + lane % kGroupRows;
     const bool in = row_is_there(st, qs, qi, row);
     double unused = 0.0;
-    float dot = in ? row_dot<SRC, float, false>(st, qs, qi, row, lane / kGroupRows, 64u / kGroupRows, unused) : 0.0f;
-    for (int o = kGroupRows; o < 64; o <<= 1)
-        dot += __shfl_xor(dot, o, 64);
+    float dot = in ? row_dot<SRC, float, false, UNROLL>(st, qs, qi, row, lane / kGroupRows, 64u / kGroupRows, unused) : 0.0f;
+    dot += __uint_as_float(xor_lane32<8>(__float_as_uint(dot)));
+    dot += __uint_as_float(xor_lane32<16>(__float_as_uint(dot)));
+    dot += __uint_as_float(xor_lane32<32>(__float_as_uint(dot)));
     if (!in)
         return neg_inf();
     return dot * fac * (st.cosine ? st.row_inv[row] : 1.0f) + (st.bias ? st.bias[row] : 0.0f);
 }
-
 __device__ __forceinline__ bool cand_before(double la, uint32_t ra, double lb, uint32_t rb) { return la > lb || (la == lb && ra < rb); }
 
 // the k-th largest of n floats in LDS (n >= k >= 1; room for whole float4), every thread gets it: rank by counting
@@ -226,6 +274,20 @@ __device__ float kth_of(const float *v, uint32_t n, uint32_t k, float *out)
 template <uint32_t THREADS>
 __device__ void order_candidates(const FinCand *cand, uint32_t n, uint32_t k, FinCand *best)
 {
+    if (n <= 64u) { // one wave, from registers
+        if (threadIdx.x < 64u) {
+            const bool mine = threadIdx.x < n;
+            const double l = mine ? cand[threadIdx.x].l : -__builtin_inf();
+            const uint32_t r = mine ? cand[threadIdx.x].row : ~0u;
+            uint32_t before = 0;
+            for (uint32_t j = 0; j < n; ++j)
+                before += cand_before(lane_d(l, j), (uint32_t)__builtin_amdgcn_readlane((int)r, (int)j), l, r) ? 1u : 0u;
+            if (mine && before < k)
+                best[before].l = l, best[before].row = r;
+        }
+        __syncthreads();
+        return;
+    }
     for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
         const double l = cand[i].l;
         const uint32_t r = cand[i].row;
@@ -275,71 +337,75 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
     const ProbUnit *units = f.units + (size_t)qi * f.n_units;
     const uint32_t n_units = JOINED ? f.n_units : st.n_pieces;
     auto unit_max = [&](uint32_t i) { return JOINED ? units[i].m : pieces[i].x; };
+    struct Part {
+        float m;
+        double s, u;
+    };
+    auto part_of = [&](uint32_t i) -> Part {
+        if (JOINED) {
+            const ProbUnit p = units[i];
+            return Part{p.m, p.s, p.u};
+        }
+        const float4 p = pieces[i];
+        return Part{p.x, (double)p.y, (double)p.z};
+    };
 
     __shared__ double red[2][WAVES];
-    __shared__ float fred[WAVES];
-    __shared__ __align__(16) float lv[kFinGroups]; // maxima: of the buckets, then of the candidate groups
+    __shared__ float lm[WAVES][64];                // the threads' maxima
+    __shared__ __align__(16) float lv[kFinGroups]; // maxima of the candidate groups (first, of the buckets)
     __shared__ uint32_t lg[kFinGroups];            // candidate groups
     __shared__ uint32_t lu[kFinGroups];            // candidate units; then candidate rows
     __shared__ FinCand cand[kFinRows + VFSX_LOG_PROBS_MAX_K];
     __shared__ FinCand best[VFSX_LOG_PROBS_MAX_K];
+    __shared__ double given_l[WAVES];              // logits of the first given rows
     __shared__ uint32_t n_lu, n_lg, n_rows, n_cand;
     __shared__ float kth;
 
     // ---- M, S, U ------------------------------------------------------------------------------------------------------------
+    // A thread's first kKeep units stay in registers, so that the usual store's are read once.
+    constexpr uint32_t kKeep = 4;
+    Part keep[kKeep];
     float m = neg_inf();
+#pragma unroll
+    for (uint32_t c = 0; c < kKeep; ++c) {
+        keep[c] = Part{neg_inf(), 0.0, 0.0};
+        if (c * THREADS < n_units && c * THREADS + tid < n_units)
+            keep[c] = part_of(c * THREADS + tid);
+        m = fmaxf(m, keep[c].m);
+    }
 #pragma unroll 4
-    for (uint32_t i = tid; i < n_units; i += THREADS)
+    for (uint32_t i = kKeep * THREADS + tid; i < n_units; i += THREADS)
         m = fmaxf(m, unit_max(i));
     const float my_max = m;
-    for (int o = 1; o < 64; o <<= 1)
-        m = fmaxf(m, __shfl_xor(m, o, 64));
-    if (lane == 0)
-        fred[wave] = m;
+    lm[wave][lane] = my_max;
     if (tid == 0)
         n_lu = n_lg = n_rows = n_cand = 0;
-    if (THREADS > kBuckets && tid < kBuckets)
-        lv[tid] = neg_inf();
     __syncthreads();
-    if (THREADS == kBuckets) {
-        lv[tid] = my_max;
-    } else {
-        // a thread's share joins bucket tid % kBuckets: the waves of one residue one after another
-        for (uint32_t r = 0; r < THREADS / kBuckets; ++r) {
-            if (tid / kBuckets == r)
-                lv[tid % kBuckets] = fmaxf(lv[tid % kBuckets], my_max);
-            __syncthreads();
-        }
-    }
-    m = fred[0];
-    for (uint32_t w = 1; w < WAVES; ++w)
-        m = fmaxf(m, fred[w]);
+    float bucket = neg_inf(); // 64 buckets, one per lane, the same in every wave
+#pragma unroll
+    for (uint32_t w = 0; w < WAVES; ++w)
+        bucket = fmaxf(bucket, lm[w][lane]);
+    m = wave_max(bucket);
     double S = 0.0, U = 0.0; // over 2^(l log2e - base), exponents in units of log 2
     const double base = piece_base64(m), L = (double)kLog2e;
+#pragma unroll
+    for (uint32_t c = 0; c < kKeep; ++c)
+        if (c * THREADS < n_units)
+            add_unit(m, keep[c].m, keep[c].s, keep[c].u, S, U);
 #pragma unroll 4
-    for (uint32_t i = tid; i < n_units; i += THREADS) {
-        if (JOINED) {
-            const ProbUnit p = units[i];
-            add_unit(m, p.m, p.s, p.u, S, U);
-        } else {
-            const float4 p = pieces[i];
-            add_unit(m, p.x, (double)p.y, (double)p.z, S, U);
-        }
+    for (uint32_t i = kKeep * THREADS + tid; i < n_units; i += THREADS) {
+        const Part p = part_of(i);
+        add_unit(m, p.m, p.s, p.u, S, U);
     }
-    for (int o = 1; o < 64; o <<= 1) {
-        S += __shfl_xor(S, o, 64);
-        U += __shfl_xor(U, o, 64);
-    }
+    S = wave_sum(S);
+    U = wave_sum(U);
     if (lane == 0) {
         red[0][wave] = S;
         red[1][wave] = U;
     }
     __syncthreads();
-    S = red[0][0], U = red[1][0];
-    for (uint32_t w = 1; w < WAVES; ++w) {
-        S += red[0][w];
-        U += red[1][w];
-    }
+    S = wave_sum(lane < WAVES ? red[0][lane] : 0.0);
+    U = wave_sum(lane < WAVES ? red[1][lane] : 0.0);
     const bool poisoned = !(S < __builtin_inf()) || U != U; // (S is about 1 or more, or 0 otherwise)
     const bool none = S == 0.0;
     const double nan = __builtin_nan("");
@@ -347,23 +413,49 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
     // ---- the k most probable rows (one at least: it is what the sums are corrected by) -----------------------------------------------
     const uint32_t k = f.k ? f.k : 1u;
     uint32_t have = 0; // rows in best[], ordered
+    const uint32_t n_early = f.log_probs ? min(f.n_given, WAVES) : 0u;
+    bool early_done = false;
     if (!poisoned && !none) {
         const float eps2 = 2.0f * qs.eps[qi];
         // first-pass logits that can be among the true k largest when `kth` is the k-th largest of some of them
         auto below = [&](float kth_value) {
             return kth_value == neg_inf() ? kth_value : kth_value - eps2 - 0x1p-21f * fmaxf(fabsf(kth_value), fabsf(m));
         };
-        // a first bound: the k-th largest of the buckets' maxima, which k groups at least reach
-        float thr = below(kth_of<THREADS>(lv, kBuckets, k, &kth));
+        // a first bound: the k-th largest of the buckets' maxima, which k groups at least reach; 64 buckets, 256 for more than 32 rows
+        float first;
+        if (k <= 32u) {
+            if (wave == 0) { // (sixteen waves that all do this take four times as long as one)
+                lv[lane] = bucket;
+                const float v = wave_kth(bucket, lv, k);
+                if (lane == 0)
+                    kth = v;
+            }
+            __syncthreads();
+            first = kth;
+        } else {
+            if (tid < kBuckets) {
+                float v = neg_inf();
+                for (uint32_t w = tid / 64u; w < WAVES; w += 4u)
+                    v = fmaxf(v, lm[w][lane]);
+                lv[tid] = v;
+            }
+            __syncthreads();
+            first = kth_of<THREADS>(lv, kBuckets, k, &kth);
+        }
+        float thr = below(first);
         // units above it -> pieces -> groups
-        for (uint32_t i = tid; i < n_units; i += THREADS) {
-            const float v = unit_max(i);
+        auto push_unit = [&](uint32_t i, float v) {
             if (v >= thr && v != neg_inf()) {
                 const uint32_t at = atomicAdd(&n_lu, 1u);
                 if (at < kFinGroups)
                     lu[at] = i;
             }
-        }
+        };
+#pragma unroll
+        for (uint32_t c = 0; c < kKeep; ++c)
+            push_unit(c * THREADS + tid, keep[c].m); // (-inf beyond the last)
+        for (uint32_t i = kKeep * THREADS + tid; i < n_units; i += THREADS)
+            push_unit(i, unit_max(i));
         __syncthreads();
         bool whole = n_lu <= kFinGroups;
         if (whole) {
@@ -400,12 +492,12 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
             const uint32_t n = n_lg;
             if (n > k) // the k-th largest group maximum: a closer bound
                 thr = fmaxf(thr, below(kth_of<THREADS>(lv, n, k, &kth)));
-            // their rows: logits in f32 (as good as the first pass') first, then those that are left in f64
+            // their rows: in f32 first, then those that are left in f64, and the given rows beside them
             const float fac = (float)(st.cosine ? 1.0 / (qs.norm[qi] * st.divide) : 1.0 / st.divide);
             for (uint32_t i = wave; i < n; i += WAVES) {
                 if (!(lv[i] >= thr))
                     continue;
-                const float l = group_logit<SRC>(st, qs, qi, lg[i], fac);
+                const float l = group_logit<SRC, (THREADS > 256u ? 8 : 4)>(st, qs, qi, lg[i], fac);
                 if (lane < kGroupRows && l >= thr && l != neg_inf()) {
                     const uint32_t at = atomicAdd(&n_rows, 1u);
                     if (at < kFinRows)
@@ -415,15 +507,21 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
             __syncthreads();
             whole = n_rows <= kFinRows;
             if (whole) {
-                const uint32_t r = n_rows;
-                for (uint32_t i = wave; i < r; i += WAVES) {
-                    const double l = row_logit<SRC>(st, qs, qi, lu[i]);
-                    if (lane == 0)
-                        cand[i].l = l, cand[i].row = lu[i];
+                for (uint32_t i = wave; i < n_rows + n_early; i += WAVES) {
+                    const bool given = i >= n_rows;
+                    const uint64_t row = given ? f.given[(size_t)qi * f.n_given + i - n_rows] - f.row_base : lu[i];
+                    const double l = row < st.n_rows ? row_logit<SRC>(st, qs, qi, (uint32_t)row) : -__builtin_inf();
+                    if (lane == 0 && given)
+                        given_l[i - n_rows] = l;
+                    else if (lane == 0)
+                        cand[i].l = l, cand[i].row = (uint32_t)row;
                 }
+                early_done = true;
                 __syncthreads();
-                order_candidates<THREADS>(cand, r, k, best);
-                have = min(r, k);
+            }
+            if (whole) {
+                order_candidates<THREADS>(cand, n_rows, k, best);
+                have = min(n_rows, k);
             }
         }
         if (!whole) {
@@ -473,20 +571,23 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
     double lse = -__builtin_inf(), entropy = 0.0;
     if (poisoned) {
         lse = entropy = nan;
-    } else if (have) {
-        const double M = best[0].l, shift = base / L - M, by = exp(shift);
+    } else if (have && wave == 0) {
+        // (exponentials in f32: their terms need no more than 2^-22 of themselves; 2^0 is 1)
+        const double M = best[0].l, shift = base / L - M, by = (double)__builtin_amdgcn_exp2f((float)(shift * L));
         double s_new = 0.0, u_new = 0.0;
-        for (uint32_t j0 = 0; j0 < have; j0 += 64u) { // (every wave the same sums, in the same order)
+        for (uint32_t j0 = 0; j0 < have; j0 += 64u) {
             const uint32_t j = j0 + lane;
             double e = 0.0, ez = 0.0, s1 = 0.0, u1 = 0.0;
             if (j < have) {
                 const uint32_t group = best[j].row / kGroupRows;
-                bool first = true;
-                for (uint32_t i = 0; i < j; ++i)
+                bool first = true; // of its group
+                for (uint32_t i = 0; i < j0; ++i)
                     first = first && best[i].row / kGroupRows != group;
+                for (uint32_t i = 0; i < 64u && j0 + i + 1u < have; ++i) // (uniform)
+                    first = first && !(i < lane && (uint32_t)__builtin_amdgcn_readlane((int)group, (int)i) == group);
                 if (first) {
                     const double z = best[j].l - M;
-                    e = exp(z);
+                    e = (double)__builtin_amdgcn_exp2f((float)(z * L));
                     ez = e * z;
                     // (the very terms that the sums have: where nothing else is there, nothing is left)
                     const float g = groups[group], pm = pieces[group / kGroupsPerPiece].x;
@@ -502,21 +603,15 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
                     }
                 }
             }
-            for (int o = 1; o < 64; o <<= 1) {
-                e += __shfl_xor(e, o, 64);
-                ez += __shfl_xor(ez, o, 64);
-                s1 += __shfl_xor(s1, o, 64);
-                u1 += __shfl_xor(u1, o, 64);
-            }
-            s_new += e;
-            u_new += ez;
-            S -= s1;
-            U -= u1;
+            s_new += wave_sum(e);
+            u_new += wave_sum(ez);
+            S -= wave_sum(s1);
+            U -= wave_sum(u1);
         }
         S = S > 0.0 ? S : 0.0;
-        const double total = S * by + s_new, weighted = (U / L + shift * S) * by + u_new;
-        lse = M + log(total);
-        entropy = log(total) - weighted / total;
+        const double total = S * by + s_new, weighted = (U / L + shift * S) * by + u_new, log_total = log(total);
+        lse = M + log_total;
+        entropy = log_total - weighted / total;
         entropy = entropy > 0.0 ? entropy : 0.0;
     }
     if (tid == 0) {
@@ -524,15 +619,21 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
             f.lse[qi] = (float)lse;
         if (f.entropy)
             f.entropy[qi] = (float)entropy;
+        red[0][0] = lse;
     }
+    __syncthreads();
+    lse = red[0][0];
 
     // ---- given rows, one wave each; the most probable rows ---------------------------------------------------------------------------
     if (f.log_probs) {
         for (uint32_t g = wave; g < f.n_given; g += WAVES) {
-            const uint64_t at = f.given[(size_t)qi * f.n_given + g] - f.row_base; // (below row_base: wraps beyond n_rows)
-            double l = -__builtin_inf();
-            if (at < st.n_rows)
-                l = row_logit<SRC>(st, qs, qi, (uint32_t)at);
+            double l;
+            if (early_done && g < n_early) {
+                l = given_l[g];
+            } else {
+                const uint64_t at = f.given[(size_t)qi * f.n_given + g] - f.row_base; // (below row_base: wraps beyond n_rows)
+                l = at < st.n_rows ? row_logit<SRC>(st, qs, qi, (uint32_t)at) : -__builtin_inf();
+            }
             if (lane == 0)
                 f.log_probs[(size_t)qi * f.n_given + g] = poisoned ? (float)nan : (l == -__builtin_inf() ? neg_inf() : (float)(l - lse));
         }

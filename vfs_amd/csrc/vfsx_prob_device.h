@@ -235,7 +235,7 @@ __device__ __forceinline__ void add_unit(float m, float m_part, double s, double
 {
     if (s == 0.0)
         return;
-    const double z = piece_base64(m_part) - piece_base64(m), e = (double)exp2f((float)z);
+    const double z = piece_base64(m_part) - piece_base64(m), e = (double)__builtin_amdgcn_exp2f((float)z);
     S += s * e;
     U += e == 0.0 ? 0.0 : (u + z * s) * e;
 }
