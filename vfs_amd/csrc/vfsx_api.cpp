@@ -2172,7 +2172,7 @@ void log_probs_impl(vfsx_corpus *c, const LogProbsArgs &a, hipStream_t s, bool c
         float4 *pieces = (float4 *)(base + w.pieces);
         float *groups = (float *)(base + w.groups);
         HIP_CHECK(few && st.n_pieces ? vfsx::launch_few_pieces(st, qs, pieces, groups, c->n_cus, s)
-                                     : vfsx::launch_prob_pieces(st, qs, pieces, groups, s));
+                                     : vfsx::launch_prob_pieces(st, qs, pieces, groups, c->n_cus, s));
         vfsx::ProbFinish f{};
         f.pieces = pieces;
         f.groups = groups;
@@ -2213,7 +2213,7 @@ void scores_f8_impl(vfsx_corpus *c, const float *d_queries, uint32_t nq, int sim
         const int bf16 = out_dtype == VFSX_SCORES_BF16;
         const bool few = prepare_queries(st, w, c->prob_work.p, d_queries + (size_t)q0 * c->dim, qn, true, bf16 != 0, qs, s);
         void *out = (char *)d_out + (size_t)q0 * ld * elem;
-        HIP_CHECK(few ? vfsx::launch_few_scores(st, qs, out, ld, bf16, c->n_cus, s) : vfsx::launch_f8_scores(st, qs, out, ld, bf16, s));
+        HIP_CHECK(few ? vfsx::launch_few_scores(st, qs, out, ld, bf16, c->n_cus, s) : vfsx::launch_f8_scores(st, qs, out, ld, bf16, c->n_cus, s));
     }
 }
 

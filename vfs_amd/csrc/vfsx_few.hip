@@ -323,10 +323,10 @@ __global__ __launch_bounds__(kFewWaves * 64, 3) void few_kernel(ProbStore st, co
                             float e[8];
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                e[i] = __uint_as_float(u[i]) * by;
-                                e[i + 4] = __uint_as_float(v[i]) * by;
+                                e[i] = __uint_as_float(u[i]);
+                                e[i + 4] = __uint_as_float(v[i]);
                             }
-                            const HalfPair r = split8(e);
+                            const HalfPair r = split8(e, by);
                             acc[t] = mfma16<SRC>(ql, __builtin_bit_cast(u32x4, r.hi), acc[t]);
                             acc[t] = mfma16<SRC>(qh, __builtin_bit_cast(u32x4, r.lo), acc[t]);
                             acc[t] = mfma16<SRC>(qh, __builtin_bit_cast(u32x4, r.hi), acc[t]);

@@ -29,6 +29,9 @@ enum ProbSource { kProbF32 = 0, kProbI8 = 1, kProbF8 = 2 };
 
 // elements of one query operand: whole blocks, which are whole K-steps of every kind
 constexpr uint32_t kQueryPad = 128;
+#if defined(__HIPCC__)
+__host__ __device__
+#endif
 inline uint32_t query_elems(uint32_t dim) { return (dim + kQueryPad - 1u) / kQueryPad * kQueryPad; }
 
 // what a pass over the store reads; the same for every query
@@ -94,15 +97,15 @@ hipError_t launch_prob_finish(const ProbStore &st, const ProbQueries &q, const P
 
 // vfsx_stream.hip: the first pass
 constexpr uint32_t kProbMaxDim = 1u << 20; // offsets inside a row-block and a block of queries stay below 2^31
-// queries the first pass computes for a launch of nq: whole tiles of 32, 64 or 128
+// queries the first pass computes for a launch of nq: whole tiles of 64 or 128
 inline uint32_t stream_query_pad(uint32_t nq)
 {
-    const uint32_t tile = nq <= 32u ? 32u : (nq <= 64u ? 64u : 128u);
+    const uint32_t tile = nq <= 64u ? 64u : 128u;
     return (nq + tile - 1u) / tile * tile;
 }
-hipError_t launch_prob_pieces(const ProbStore &st, const ProbQueries &q, float4 *pieces, float *groups, hipStream_t s);
+hipError_t launch_prob_pieces(const ProbStore &st, const ProbQueries &q, float4 *pieces, float *groups, uint32_t n_cus, hipStream_t s);
 // out[nq][ld]: f32 (bf16 = 0) or bf16
-hipError_t launch_f8_scores(const ProbStore &st, const ProbQueries &q, void *out, uint64_t ld, int bf16, hipStream_t s);
+hipError_t launch_f8_scores(const ProbStore &st, const ProbQueries &q, void *out, uint64_t ld, int bf16, uint32_t n_cus, hipStream_t s);
 
 // vfsx_few.hip: the first pass for up to 8 queries; prepares them itself
 constexpr uint32_t kFewQueries = 8;

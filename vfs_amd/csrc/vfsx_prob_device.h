@@ -127,17 +127,21 @@ struct HalfPair {
     f16x8 hi, lo;
 };
 
-__device__ __forceinline__ HalfPair split8(const float *x)
+// 8 values times `by` (a power of two) as hi + lo: hi is the rounded product, lo the rounded rest, and both are exact before their rounding.
+// Of the rest, multiply, subtract and round are one instruction.
+__device__ __forceinline__ HalfPair split8(const float *x, float by)
 {
     HalfPair r;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-        const f32x2 v = {x[i], x[i + 1]};
-        const f16x2 h = __builtin_convertvector(v, f16x2);
-        const f32x2 rest = {__builtin_fmaf((float)h[0], -1.0f, x[i]), __builtin_fmaf((float)h[1], -1.0f, x[i + 1])};
-        const f16x2 l = __builtin_convertvector(rest, f16x2);
+        uint32_t hi;
+        const f32x2 v = {x[i] * by, x[i + 1] * by};
+        hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+        asm("" : "+v"(hi)); // (one value for both uses: the compiler would round twice)
+        const f16x2 h = __builtin_bit_cast(f16x2, hi);
         r.hi[i] = h[0], r.hi[i + 1] = h[1];
-        r.lo[i] = l[0], r.lo[i + 1] = l[1];
+        r.lo[i] = (_Float16)__builtin_fmaf(x[i], by, -(float)h[0]);
+        r.lo[i + 1] = (_Float16)__builtin_fmaf(x[i + 1], by, -(float)h[1]);
     }
     return r;
 }

@@ -12,16 +12,20 @@
 //              than its neighbour is lost; seen with products of powers of two), so its sums are good to 2^-13 of a group's largest
 //              product (1.5e-5 of a result, by the norm): fine for scores that are rounded to bf16 (2^-9), not for f32 results.
 //
-// One wave owns a row-block (64 rows = two 32-row tiles of the A operand) and 32 NT queries.  Its rows go global -> VGPR (16 bytes per
-// lane and load, 1 KiB contiguous per wave as rb64 has them), one K-step ahead; nobody else needs them, so they never pass
-// through LDS.  The queries (B operand) are shared by the WAVES waves of a workgroup: a ring of three LDS slots filled by
-// buffer_load ... lds two K-steps ahead, one barrier per K-step.
+// A workgroup is 4 (or 2) waves: 256 (128) rows by 32 NT queries.  A wave owns a row-block, 64 rows = two A tiles, and all the queries: its rows go
+// global -> VGPR, PF K-steps ahead, are converted there once, and nobody else needs them.  The queries (B operand) are shared: a ring of
+// LDS slots filled by buffer_load ... lds, kSlots - 1 K-steps ahead, one barrier per K-step.  (One A tile per wave and twice the queries
+// reads LDS for every product: e4m3 rows then wait for it, 39 % of the matrix cores.)  Two workgroups per CU (NT = 4: 128 accumulators of
+// 256 registers), so that one's epilogue runs beside the other's products; each walks a list of tiles, and the loads run on across
+// the border from one tile to the next.  (One tile per workgroup, and the rows' registers copied at the end of a K-step -- which waits for
+// them there: 5 us until the first product of a tile of 27 us, 2.1 us a K-step of 0.9 us of products.)
 //
 // Row order inside a 32-row tile: matrix row 8 a + 4 h + b holds store row 16 h + 4 a + b, so that the 16 accumulators of a lane (matrix
 // rows 8 a + 4 h + b of its half h) are 16 consecutive rows of the store: a group's maximum and its share of the sums need no
 // other lane, and a lane writes 16 consecutive scores.
 #include <hip/hip_runtime.h>
 
+#include "vfsx_device.h"
 #include "vfsx_internal.h"
 #include "vfsx_prob.h"
 #include "vfsx_prob_device.h"
@@ -33,199 +37,224 @@ namespace vfsx {
 namespace {
 
 enum { kF8Raw = 3 }; // beside ProbSource
-// What one K-step is.  Rows: kLoads loads of 16 bytes per lane (two tiles, each lane half every other chunk).  Queries: kQChunks chunks of
-// 16 bytes in kQParts parts (hi, lo), three slots of which leave room for two workgroups per CU.
-template <int SRC, int NT>
+
+// What one K-step is: kSlotData bytes of queries, as many elements as that is for 32 NT queries.  WAVES row-blocks per workgroup: four, or
+// two where there are few tiles; then nothing but more loads on their way hides a load's latency, and there are registers for them.
+template <int SRC, int NT, int WAVES>
 struct Step {
-    static constexpr uint32_t kElems = SRC == kProbF32 ? 32u : (SRC == kF8Raw ? 128u : (SRC == kProbI8 && NT == 4 ? 32u : 64u));
-    static constexpr uint32_t kChunks = kElems / (SRC == kProbF32 ? 4u : 16u);
-    static constexpr uint32_t kLoads = kChunks;
-    static constexpr uint32_t kQChunks = SRC == kF8Raw ? 8u : kElems / 8u;
-    static constexpr uint32_t kQParts = SRC == kProbF32 || SRC == kProbI8 ? 2u : 1u;
-    static constexpr uint32_t kSlotBytes = kQChunks * kQParts * NT * 512u;
+    static constexpr uint32_t kQParts = SRC == kProbF32 || SRC == kProbI8 ? 2u : 1u; // hi, lo
+    static constexpr uint32_t kQBytes = SRC == kF8Raw ? 1u : 2u;                      // of an element of a part
+    static constexpr uint32_t kSlotData = (SRC == kProbI8 ? 4096u : 2048u) * NT * (WAVES == 2 ? 2u : 1u);
+    static constexpr uint32_t kElems = kSlotData / (32u * NT * kQParts * kQBytes);
+    static constexpr uint32_t kQChunks = kElems * kQBytes / 16u;
+    static constexpr uint32_t kChunks = kElems / (SRC == kProbF32 ? 4u : 16u); // of a row
+    static constexpr uint32_t kTileLoads = kChunks / 2u;                       // per lane and A tile: half of a row's chunks each
+    static constexpr uint32_t kLoads = 2u * kTileLoads;
+    static constexpr uint32_t kRowWords = SRC == kProbI8 ? 0u : 2u;            // and a dword per tile: the row's scale, or four exponents
+    static constexpr uint32_t kPieces = kSlotData / 1024u;                     // 1 KiB each: one copy by one wave
+    static constexpr uint32_t kExpDma = SRC == kF8Raw ? 1u : 0u;               // raw: the queries' exponents
+    // vector memory instructions of a wave and K-step
+    static constexpr uint32_t kDma = kPieces / WAVES + kExpDma, kA = kLoads + kRowWords;
+    static constexpr uint32_t kSlotBytes = kSlotData + kExpDma * 1024u;
+    static constexpr uint32_t kSlots = SRC == kProbI8 ? 3u : 5u;
+    static constexpr uint32_t kPf = kLoads <= 2u || (WAVES == 2 && kLoads == 4u) ? 4u : 3u;
+    static constexpr uint32_t kWavesPerSimd = WAVES == 2 || NT == 4 ? 2u : 3u;
+    static constexpr uint32_t kWgPerCu = kWavesPerSimd * 4u / WAVES;
+    // The queries of a K-step are here when at most this many younger instructions are on their way: the copies of the kSlots - 2 younger
+    // slots and the rows' loads issued since (in the first steps those of the prologue, at least min(kPf, kSlots - 2) of them; anything
+    // else that was issued since makes this stricter).
+    static constexpr uint32_t kYounger = (kSlots - 2u) * kDma + (kPf < kSlots - 2u ? kPf : kSlots - 2u) * kA;
+    static_assert(kElems >= 16u && kElems <= kF8Block && kPieces % WAVES == 0 && kYounger < 64u, "a K-step");
 };
 
 template <int SRC, int NT, int WAVES, int EPI>
-__global__ __launch_bounds__(WAVES * 64, NT == 4 ? 2 : (NT == 2 ? 3 : 4)) void stream_kernel(ProbStore st, ProbQueries qs, StreamOut out, uint32_t n_rowtiles,
-                                                                            uint32_t n_qtiles, uint32_t q_group)
+__global__ __launch_bounds__(WAVES * 64, (Step<SRC, NT, WAVES>::kWavesPerSimd)) void stream_kernel(ProbStore st, ProbQueries qs, StreamOut out,
+                                                                                                  uint32_t n_rowtiles, uint32_t n_qtiles)
 {
-    using S = Step<SRC, NT>;
+    using S = Step<SRC, NT, WAVES>;
     constexpr bool kIsF8 = SRC == kProbF8 || SRC == kF8Raw;
-    constexpr uint32_t kSlots = 3, kSlotBytes = S::kSlotBytes, kPieces1k = kSlotBytes / 1024u;
-    constexpr uint32_t kDma = (kPieces1k + WAVES - 1u) / WAVES; // per wave and slot (the last may be redundant)
-    static_assert(NT == 1 || NT == 2 || NT == 4, "query tiles");
-    __shared__ __align__(1024) uint8_t ring[kSlots][kSlotBytes];
+    constexpr uint32_t kSlots = S::kSlots, PF = S::kPf;
+    __shared__ __align__(1024) uint8_t ring[kSlots * S::kSlotBytes];
     __shared__ __align__(16) float row_mul[WAVES][64], row_add[WAVES][64]; // epilogue: each wave its own rows
-
     const uint32_t lane = threadIdx.x & 63u, h = lane >> 5, r32 = lane & 31u;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t perm = 16u * ((r32 >> 2) & 1u) + 4u * (r32 >> 3) + (r32 & 3u); // store row (in its tile of 32) of matrix row r32
 
-    // Work items (row tile, query tile).  Workgroups with the same id % 8 share an XCD and its L2: they take whole groups of q_group query
-    // tiles for one row tile next to one another, so the rows come from memory once per group.
-    const uint32_t xcd = blockIdx.x & 7u, within = blockIdx.x >> 3;
-    const uint32_t groups_q = (n_qtiles + q_group - 1u) / q_group;
-    const uint32_t rt = (within / q_group / groups_q) * 8u + xcd;
-    const uint32_t qt = (within / q_group % groups_q) * q_group + within % q_group;
-    if (rt >= n_rowtiles || qt >= n_qtiles)
+    // Tiles.  Workgroups with the same id % 8 share an XCD and its L2.  An XCD owns every eighth row tile; its list goes through groups of (up
+    // to) 8 query tiles, in a group row tile by row tile, so that its workgroups read few row tiles and few query tiles at a time, each
+    // several times from L2.
+    const uint32_t xcd = blockIdx.x & 7u, place = blockIdx.x >> 3, places = gridDim.x >> 3;
+    const uint32_t my_rowtiles = n_rowtiles > xcd ? (n_rowtiles - xcd + 7u) / 8u : 0u;
+    const uint32_t n_tiles = my_rowtiles * n_qtiles;
+    if (place >= n_tiles)
         return; // (the whole workgroup)
+    const uint32_t my_tiles = (n_tiles - place + places - 1u) / places;
+    struct Tile {
+        uint32_t rt, qt;
+    };
+    auto tile_at = [&](uint32_t i) -> Tile { // the i-th of this workgroup (past the end: the last again)
+        const uint32_t t = place + places * min(i, my_tiles - 1u);
+        const uint32_t group = min(t / (8u * my_rowtiles), (n_qtiles - 1u) / 8u), in_group = t - group * 8u * my_rowtiles;
+        const uint32_t width = min(8u, n_qtiles - group * 8u);
+        return Tile{xcd + 8u * (in_group / width), group * 8u + in_group % width};
+    };
 
-    const uint32_t n_rb = (st.n_rows + 63u) / 64u, rb = rt * WAVES + wave;
-    const bool active = rb < n_rb;
+    const uint32_t n_rb = (st.n_rows + 63u) / 64u, n_step = (st.dim + S::kElems - 1u) / S::kElems;
     const uint32_t row_chunks = kIsF8 ? st.f8_chunks : st.d_chunks;
-    const uint4 *a_base = (kIsF8 ? st.f8 : st.rows) + (size_t)(active ? rb : 0u) * row_chunks * 64u;
-    // bounded by the row-block: chunks beyond a row's last read as zeros
-    const __amdgpu_buffer_rsrc_t a_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)a_base, 0, active ? row_chunks * 1024u : 0u, 0x00020000);
-    const uint32_t n_step = (st.dim + S::kElems - 1u) / S::kElems;
+    const uint4 *rows = kIsF8 ? st.f8 : st.rows;
 
-    // queries: 64-query blocks of 1 KiB pieces, padded to kQueryPad elements
-    const uint32_t q_block_bytes = (st.dim + kQueryPad - 1u) / kQueryPad * kQueryPad * (SRC == kF8Raw ? 64u : 128u * S::kQParts);
-    const uint8_t *b_base = (const uint8_t *)qs.operand + (size_t)(NT == 4 ? qt * 2u : (NT == 2 ? qt : qt >> 1)) * q_block_bytes;
-    const __amdgpu_buffer_rsrc_t b_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)b_base, 0, 0xffffffffu, 0x00020000);
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)&ring[0][0];
-
+    // ---- queries: 64-query blocks of 1 KiB pieces, padded to kQueryPad elements ------------------------------------------------------------
+    const uint32_t q_block_bytes = query_elems(st.dim) * 64u * S::kQBytes * S::kQParts;
+    const __amdgpu_buffer_rsrc_t e_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)qs.q8_exp, 0, 0xffffffffu, 0x00020000);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)&ring[0];
+    uint32_t b_item = 0, b_step = 0, b_slot = 0, b_qt = 0;
+    __amdgpu_buffer_rsrc_t b_rsrc;
+    auto next_queries = [&] {
+        b_step = 0;
+        b_qt = tile_at(b_item++).qt;
+        b_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)qs.operand + (size_t)b_qt * (NT / 2u) * q_block_bytes), 0, 0xffffffffu,
+                                                   0x00020000);
+    };
+    next_queries();
+    auto dma = [&](__amdgpu_buffer_rsrc_t rsrc, uint32_t dst, uint32_t voff, uint32_t soff) {
+        asm volatile("" : "+s"(dst)); // (the compiler must not tie this to later reads of `ring`: it would drain the ring)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(uintptr_t)dst, 16, (int)voff, (int)soff, 0, 0);
+    };
     // slot layout [tile nt][chunk][part][32 queries][16 B].  One DMA moves 1 KiB = two runs of 512 B: chunk * part pairs (2 j, 2 j + 1) of one
     // 32-query tile; lane >> 5 picks the pair's member.
-    auto stage_queries = [&](uint32_t step, uint32_t slot) {
+    auto stage_queries = [&] {
+        const uint32_t slot = lds0 + b_slot * S::kSlotBytes;
 #pragma unroll
-        for (uint32_t i = 0; i < kDma; ++i) {
-            const uint32_t piece = min(wave * kDma + i, kPieces1k - 1u); // (redundant copies keep the count the same in every wave)
-            constexpr uint32_t per_tile = S::kQChunks * S::kQParts / 2u;
-            const uint32_t nt = piece / per_tile, pair = piece % per_tile;
-            const uint32_t block = NT == 4 ? nt >> 1 : 0u, half = NT == 1 ? qt & 1u : nt & 1u;
-            const uint32_t voff = h * 1024u + half * 512u + r32 * 16u;
-            const uint32_t soff = block * q_block_bytes + (step * S::kQChunks * S::kQParts + 2u * pair) * 1024u;
-            uint32_t dst = lds0 + slot * kSlotBytes + piece * 1024u;
-            asm volatile("" : "+s"(dst)); // (the compiler must not tie this to later reads of `ring`: it would drain the ring)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(b_rsrc, (__attribute__((address_space(3))) void *)(uintptr_t)dst, 16, (int)voff, (int)soff, 0, 0);
+        for (uint32_t i = 0; i < S::kPieces / WAVES; ++i) {
+            const uint32_t piece = wave * (S::kPieces / WAVES) + i;
+            constexpr uint32_t per_tile = S::kPieces / NT;
+            const uint32_t tile32 = piece / per_tile, pair = piece % per_tile;
+            dma(b_rsrc, slot + piece * 1024u, h * 1024u + r32 * 16u,
+                (tile32 >> 1) * q_block_bytes + (tile32 & 1u) * 512u + (b_step * S::kQChunks * S::kQParts + 2u * pair) * 1024u);
         }
+        if (S::kExpDma) { // (every wave the same 1 KiB) a dword of exponents for each query: 16 bytes of a 64-query block per lane
+            const uint32_t word = b_step * S::kElems / (4u * kF8Block);
+            const uint32_t block = min(b_qt * (NT / 2u) + (lane >> 4), (qs.nq - 1u) / 64u); // (four blocks' worth; the tile has NT / 2)
+            dma(e_rsrc, slot + S::kSlotData, (block * st.f8_words + word) * 256u + (lane & 15u) * 16u, 0);
+        }
+        if (++b_slot == kSlots)
+            b_slot = 0;
+        if (++b_step == n_step)
+            next_queries();
     };
-    u32x4 a_next[S::kLoads];
-    auto load_rows = [&](uint32_t step, u32x4 *a) {
+    // ---- rows --------------------------------------------------------------------------------------------------------------------------------
+    struct Ahead {
+        u32x4 a[S::kLoads];
+        uint32_t word[2];
+    };
+    // the row-block's chunks from this K-step on: chunks beyond a row's last read as zeros, and past the last tile nothing is read
+    uint32_t a_item = 0, a_step = 0, a_chunk = 0; // (a_chunk: 1 KiB, or nothing)
+    const uint4 *a_from = nullptr;
+    const uint32_t *a_words = nullptr;
+    auto next_rows = [&] {
+        const uint32_t my_rb = tile_at(a_item).rt * WAVES + wave, rb = min(my_rb, n_rb - 1u);
+        a_step = 0;
+        a_from = rows + (size_t)rb * row_chunks * 64u;
+        a_chunk = my_rb < n_rb && a_item < my_tiles ? 1024u : 0u;
+        a_words = SRC == kProbF32 ? (const uint32_t *)st.row_scale + rb * 64u : st.f8_exp + (size_t)rb * st.f8_words * 64u;
+        ++a_item;
+    };
+    next_rows();
+    const uint32_t a_lane = ((SRC == kProbI8 || SRC == kProbF8 ? 1u : 2u) * h * 64u + perm) * 16u;
+    auto load_rows = [&](Ahead &x) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)a_from, 0, (row_chunks - a_step * S::kChunks) * a_chunk, 0x00020000);
 #pragma unroll
         for (uint32_t i = 0; i < S::kLoads; ++i) {
-            const uint32_t mt = i / (S::kLoads / 2u), j = i % (S::kLoads / 2u);
+            const uint32_t mt = i / S::kTileLoads, j = i % S::kTileLoads;
             // f32: chunks 4 s + 2 h, 4 s + 2 h + 1 of K-slice s (16 elements);  raw e4m3: the same of K-slice s (64 elements);
             // int8 and e4m3: chunk 2 j + h, two K-slices of 16 elements out of one 16-byte chunk per lane half
-            const uint32_t c = SRC == kProbI8 || SRC == kProbF8 ? 2u * j + h : 4u * (j >> 1) + 2u * h + (j & 1u);
-            const uint32_t off = (step * S::kChunks + c) * 1024u + (mt * 32u + perm) * 16u;
-            a[i] = __builtin_amdgcn_raw_buffer_load_b128(a_rsrc, (int)off, 0, 0);
+            const uint32_t c = SRC == kProbI8 || SRC == kProbF8 ? 2u * j : 4u * (j >> 1) + (j & 1u); // (+ h's part: a_lane)
+            x.a[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(a_lane + c * 1024u + mt * 512u), 0, 0);
         }
+        const uint32_t *words = a_words + (kIsF8 ? a_step * S::kElems / (4u * kF8Block) * 64u : 0u);
+#pragma unroll
+        for (uint32_t mt = 0; mt < S::kRowWords; ++mt)
+            x.word[mt] = words[mt * 32u + perm];
+        a_from += S::kChunks * 64u;
+        if (++a_step == n_step)
+            next_rows();
     };
 
     f32x16 acc[2][NT];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+    for (int nt = 0; nt < NT; ++nt)
+        acc[0][nt] = acc[1][nt] = f32x16{};
+    Ahead ahead[PF];
+    // the order of issue is what the counted wait below relies on: slot by slot, rows by rows
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                acc[mt][nt][i] = 0.0f;
-
-    float a_scale[2] = {1.0f, 1.0f};
-    if (SRC == kProbF32) {
-#pragma unroll
-        for (uint32_t mt = 0; mt < 2u; ++mt)
-            a_scale[mt] = st.row_scale[(active ? rb : 0u) * 64u + mt * 32u + perm];
+    for (uint32_t i = 0; i < (kSlots - 1u > PF ? kSlots - 1u : PF); ++i) {
+        if (i < kSlots - 1u)
+            stage_queries();
+        asm volatile("" ::: "memory");
+        if (i < PF)
+            load_rows(ahead[i]);
+        asm volatile("" ::: "memory");
     }
-    uint32_t a_exp[2] = {0, 0}, b_exp[NT] = {};
-    const uint32_t *a_exp_at = nullptr, *b_exp_at = nullptr;
-    if (kIsF8) {
-        a_exp_at = st.f8_exp + (size_t)(active ? rb : 0u) * st.f8_words * 64u + perm;
-        if (SRC == kF8Raw)
-            b_exp_at = qs.q8_exp + (size_t)(NT == 4 ? qt * 2u : (NT == 2 ? qt : qt >> 1)) * st.f8_words * 64u + (NT == 1 ? (qt & 1u) * 32u : 0u) + r32;
-    }
-
-    stage_queries(0, 0);
-    asm volatile("" ::: "memory");
-    stage_queries(n_step > 1u ? 1u : 0u, 1);
-    asm volatile("" ::: "memory");
-    load_rows(0, a_next);
-    asm volatile("" ::: "memory");
 
     uint32_t slot = 0;
-    for (uint32_t step = 0; step < n_step; ++step) {
-        u32x4 a[S::kLoads];
-#pragma unroll
-        for (uint32_t i = 0; i < S::kLoads; ++i)
-            a[i] = a_next[i];
-        // the queries of this step are here (all but the youngest: the next step's queries and this step's rows), for every wave;
-        // and every wave is done reading the slot that is filled next
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kDma + S::kLoads) : "memory");
+    auto k_step = [&](Ahead &x, uint32_t step) __attribute__((always_inline)) {
+        // the queries of this step are here; then for every wave, and every wave is done reading the slot that is filled next
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(S::kYounger) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        const uint32_t fill = slot == 0u ? 2u : slot - 1u;
-        stage_queries(min(step + 2u, n_step - 1u), fill);
+        stage_queries();
         asm volatile("" ::: "memory");
-        load_rows(min(step + 1u, n_step - 1u), a_next);
-        asm volatile("" ::: "memory");
-        constexpr uint32_t kStepsPerWord = 4u * kF8Block / S::kElems; // of a dword of scales
-        if (kIsF8 && step % kStepsPerWord == 0u) {
-            const uint32_t word = step / kStepsPerWord;
-#pragma unroll
-            for (uint32_t mt = 0; mt < 2u; ++mt)
-                a_exp[mt] = a_exp_at[(size_t)word * 64u + mt * 32u];
-            if (SRC == kF8Raw) {
-#pragma unroll
-                for (uint32_t nt = 0; nt < NT; ++nt)
-                    b_exp[nt] = b_exp_at[((size_t)(nt >> 1) * st.f8_words + word) * 64u + (nt & 1u) * 32u];
-            }
-        }
-        const uint8_t *q_slot = ring[slot];
+        const uint8_t *q_slot = ring + slot * S::kSlotBytes;
         auto q_frag = [&](uint32_t nt, uint32_t chunk, uint32_t part) {
             return *(const u32x4 *)(q_slot + ((nt * S::kQChunks + chunk) * S::kQParts + part) * 512u + r32 * 16u);
         };
         if constexpr (SRC == kF8Raw) {
-            const uint32_t sh = 8u * (step & 3u);
+            const uint32_t sh = 8u * ((step * S::kElems / kF8Block) & 3u);
 #pragma unroll
-            for (uint32_t s = 0; s < 2u; ++s) {
+            for (uint32_t s = 0; s < S::kElems / 64u; ++s) {
                 i32x8 fa[2];
 #pragma unroll
                 for (uint32_t mt = 0; mt < 2u; ++mt) {
-                    const u32x4 p = a[mt * 4u + s * 2u], q = a[mt * 4u + s * 2u + 1u];
-                    fa[mt] = i32x8{(int)p[0], (int)p[1], (int)p[2], (int)p[3], (int)q[0], (int)q[1], (int)q[2], (int)q[3]};
+                    const u32x4 u = x.a[mt * S::kTileLoads + 2u * s], v = x.a[mt * S::kTileLoads + 2u * s + 1u];
+                    fa[mt] = i32x8{(int)u[0], (int)u[1], (int)u[2], (int)u[3], (int)v[0], (int)v[1], (int)v[2], (int)v[3]};
                 }
 #pragma unroll
                 for (uint32_t nt = 0; nt < NT; ++nt) {
                     const u32x4 p = q_frag(nt, 4u * s + 2u * h, 0), q = q_frag(nt, 4u * s + 2u * h + 1u, 0);
                     const i32x8 fb = {(int)p[0], (int)p[1], (int)p[2], (int)p[3], (int)q[0], (int)q[1], (int)q[2], (int)q[3]};
+                    const uint32_t e = *(const uint32_t *)(q_slot + S::kSlotData + (nt * 32u + r32) * 4u);
 #pragma unroll
                     for (uint32_t mt = 0; mt < 2u; ++mt)
-                        acc[mt][nt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[mt], fb, acc[mt][nt], 0, 0, 0,
-                                                                                      (int)(a_exp[mt] >> sh), 0, (int)(b_exp[nt] >> sh));
+                        acc[mt][nt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[mt], fb, acc[mt][nt], 0, 0, 0, (int)(x.word[mt] >> sh),
+                                                                                      0, (int)(e >> sh));
                 }
             }
         } else {
             constexpr uint32_t kSlices = S::kElems / 16u;
-            float f8_scale[2] = {}; // this step's block
-            if (SRC == kProbF8) {
-#pragma unroll
-                for (uint32_t mt = 0; mt < 2u; ++mt)
-                    f8_scale[mt] = __uint_as_float(((a_exp[mt] >> (8u * (step / (kF8Block / S::kElems) & 3u))) & 255u) << 23);
-            }
 #pragma unroll
             for (uint32_t s = 0; s < kSlices; ++s) {
                 u32x4 ah[2], al[2];
 #pragma unroll
                 for (uint32_t mt = 0; mt < 2u; ++mt) {
+                    const u32x4 *a = x.a + mt * S::kTileLoads;
                     if constexpr (SRC == kProbF32) {
-                        const u32x4 p = a[mt * 4u + s * 2u], q = a[mt * 4u + s * 2u + 1u];
-                        float x[8];
+                        const float by = __uint_as_float(x.word[mt]);
+                        float e[8];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            x[i] = __uint_as_float(p[i]) * a_scale[mt];
-                            x[i + 4] = __uint_as_float(q[i]) * a_scale[mt];
+                            e[i] = __uint_as_float(a[2u * s][i]);
+                            e[i + 4] = __uint_as_float(a[2u * s + 1u][i]);
                         }
-                        const HalfPair v = split8(x);
+                        const HalfPair v = split8(e, by);
                         ah[mt] = __builtin_bit_cast(u32x4, v.hi);
                         al[mt] = __builtin_bit_cast(u32x4, v.lo);
                     } else {
-                        const u32x4 p = a[mt * (S::kLoads / 2u) + (s >> 1)];
-                        const uint32_t lo = p[(s & 1u) * 2u], hi = p[(s & 1u) * 2u + 1u];
+                        const uint32_t lo = a[s >> 1][(s & 1u) * 2u], hi = a[s >> 1][(s & 1u) * 2u + 1u];
                         if constexpr (SRC == kProbI8)
                             ah[mt] = __builtin_bit_cast(u32x4, halves8(lo, hi));
                         else
-                            ah[mt] = bf16_of_e4m3(lo, hi, f8_scale[mt]);
+                            ah[mt] = bf16_of_e4m3(lo, hi,
+                                                  __uint_as_float(((x.word[mt] >> (8u * ((step * S::kElems / kF8Block) & 3u))) & 255u) << 23));
                     }
                 }
                 // the 8 elements a lane half supplies: f32 16 s + 8 h ..;  int8, e4m3 16 (2 (s / 2) + h) + 8 (s % 2) ..
@@ -236,196 +265,252 @@ __global__ __launch_bounds__(WAVES * 64, NT == 4 ? 2 : (NT == 2 ? 3 : 4)) void s
                     u32x4 bl = bh;
                     if (S::kQParts == 2u)
                         bl = q_frag(nt, qc, 1);
+                    // (the two A tiles in turn: no product waits for the one before it)
+                    if (S::kQParts == 2u) {
 #pragma unroll
-                    for (uint32_t mt = 0; mt < 2u; ++mt) {
-                        if (S::kQParts == 2u)
+                        for (uint32_t mt = 0; mt < 2u; ++mt)
                             acc[mt][nt] = mfma16<SRC>(ah[mt], bl, acc[mt][nt]);
-                        if (SRC == kProbF32)
-                            acc[mt][nt] = mfma16<SRC>(al[mt], bh, acc[mt][nt]);
-                        acc[mt][nt] = mfma16<SRC>(ah[mt], bh, acc[mt][nt]);
                     }
+                    if (SRC == kProbF32) {
+#pragma unroll
+                        for (uint32_t mt = 0; mt < 2u; ++mt)
+                            acc[mt][nt] = mfma16<SRC>(al[mt], bh, acc[mt][nt]);
+                    }
+#pragma unroll
+                    for (uint32_t mt = 0; mt < 2u; ++mt)
+                        acc[mt][nt] = mfma16<SRC>(ah[mt], bh, acc[mt][nt]);
                 }
             }
         }
-        slot = slot == 2u ? 0u : slot + 1u;
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // no copy into LDS may outlive the workgroup
-    if (!active)
-        return;
+        // The order of the step: fragments ahead of the products that use them, so that no product waits for LDS (left to itself the compiler
+        // reads each fragment right before its products).
+        if constexpr (SRC == kF8Raw) {
+            constexpr int kTiles = NT * (int)(S::kElems / 64u); // two fragments and a dword of exponents, two products of 64 cycles each
+            __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+            for (int i = 0; i < kTiles - 2; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        } else {
+            constexpr int kReads = NT * (int)(S::kQParts * S::kElems / 16u);
+            constexpr int kPer2 = SRC == kProbF32 ? 6 : 4; // products for two fragments
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 0; i < kReads / 2 - 2; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, kPer2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * kPer2, 0);
+        }
+        // (nothing is read here: the products stay in their K-step instead of sinking to where the accumulators are used)
+#pragma unroll
+        for (uint32_t nt = 0; nt < NT; ++nt)
+            asm volatile("" : "+v"(acc[0][nt]), "+v"(acc[1][nt]));
+        load_rows(x);
+        asm volatile("" ::: "memory");
+        slot = slot + 1u == kSlots ? 0u : slot + 1u;
+    };
 
-    // ---- epilogue: lane = query (column) r32 of tile nt; acc[mt][nt][i] = row 64 rb + 32 mt + 16 h + i ----------------------------------
-    const uint32_t q0 = qt * (32u * NT) + r32;
-    if constexpr (EPI == kPieces) {
-        // Who is there: one row of the block per lane.  Blocks with rows that are not there, or with a bias so low that its logit leaves
-        // the range of the exponent below, take the longer way (`masked`).
-        const uint32_t my = rb * 64u + lane;
-        bool gone = my >= st.n_rows, low = false;
-        float my_mul = 1.0f, my_add = 0.0f;
-        if (!gone) {
-            my_add = st.bias ? st.bias[my] : 0.0f;
-            my_mul = st.cosine ? st.row_inv[my] : 1.0f;
-            gone = my_add == neg_inf() || (st.cosine && my_mul < 0.0f);
-            low = fabsf(my_add) > 1e30f;
-            if (SRC == kProbF32) // / 2^a
-                my_mul *= __uint_as_float((254u << 23) - __float_as_uint(st.row_scale[my]));
+    for (uint32_t item = 0; item < my_tiles; ++item) {
+        uint32_t step = 0;
+        for (; step + PF <= n_step; step += PF) {
+#pragma unroll
+            for (uint32_t p = 0; p < PF; ++p)
+                k_step(ahead[p], step + p);
         }
-        row_mul[wave][lane] = my_mul;
-        row_add[wave][lane] = my_add;
-        const bool masked = __any(gone || low);
-        const uint64_t gone_rows = __ballot(gone);
-        const uint32_t gone_mine = (uint32_t)((gone_rows >> (16u * h)) & 0xffffu) | (uint32_t)((gone_rows >> (32u + 16u * h)) & 0xffffu) << 16;
+        const uint32_t rest = n_step - step; // < PF
 #pragma unroll
-        for (uint32_t nt = 0; nt < NT; ++nt) {
-            const uint32_t qi = q0 + nt * 32u;
-            const bool mine = qi < qs.nq;
-            const float fac = mine ? qs.fac[qi] : 0.0f;
-            float top[2][2] = {{neg_inf(), neg_inf()}, {neg_inf(), neg_inf()}}, s = 0.0f, t = 0.0f, m;
-            auto logit = [&](uint32_t mt, uint32_t i) { // (the same address in all lanes of a half)
-                const uint32_t at = mt * 32u + h * 16u + i;
-                return __builtin_fmaf(acc[mt][nt][i], fac * row_mul[wave][at], row_add[wave][at]);
-            };
-            auto is_gone = [&](uint32_t mt, uint32_t i) { return (gone_mine >> (16u * mt + i)) & 1u; };
-            if (!masked) {
+        for (uint32_t p = 0; p + 1u < PF; ++p)
+            if (p < rest)
+                k_step(ahead[p], step + p);
+        // the next tile starts with ahead[0] again
+        for (uint32_t i = 0; i < rest; ++i) {
+            const Ahead first = ahead[0];
 #pragma unroll
-                for (uint32_t mt = 0; mt < 2u; ++mt)
-#pragma unroll
-                    for (uint32_t i = 0; i < 16u; ++i) {
-                        acc[mt][nt][i] = logit(mt, i);
-                        top[mt][i >> 3] = fmaxf(top[mt][i >> 3], acc[mt][nt][i]);
-                    }
-                m = fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[1][0], top[1][1]));
-                m = fmaxf(m, __shfl_xor(m, 32, 64));
-                const float base = piece_base(m);
-#pragma unroll
-                for (uint32_t mt = 0; mt < 2u; ++mt)
-#pragma unroll
-                    for (uint32_t i = 0; i < 16u; ++i) {
-                        const float z = __builtin_fmaf(acc[mt][nt][i], kLog2e, -base), e = __builtin_amdgcn_exp2f(z);
-                        s += e;
-                        t = __builtin_fmaf(e, z, t);
-                    }
-            } else {
-#pragma unroll
-                for (uint32_t mt = 0; mt < 2u; ++mt)
-#pragma unroll
-                    for (uint32_t i = 0; i < 16u; ++i) {
-                        acc[mt][nt][i] = is_gone(mt, i) ? neg_inf() : logit(mt, i);
-                        top[mt][i >> 3] = fmaxf(top[mt][i >> 3], acc[mt][nt][i]);
-                    }
-                m = fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[1][0], top[1][1]));
-                m = fmaxf(m, __shfl_xor(m, 32, 64));
-                const float base = piece_base(m);
-                const bool huge = piece_is_huge(m);
-#pragma unroll
-                for (uint32_t mt = 0; mt < 2u; ++mt)
-#pragma unroll
-                    for (uint32_t i = 0; i < 16u; ++i) {
-                        const float l = acc[mt][nt][i];
-                        const float z = huge ? (l - m) * kLog2e : __builtin_fmaf(l, kLog2e, -base);
-                        const float e = __builtin_amdgcn_exp2f(z);
-                        // (a row there whose logit is infinite spoils the sums; a very low finite one adds nothing)
-                        s += is_gone(mt, i) ? 0.0f : (fabsf(l) < __builtin_inff() ? e : __builtin_nanf(""));
-                        t += is_gone(mt, i) || e == 0.0f ? 0.0f : e * z;
-                    }
-            }
-            s += __shfl_xor(s, 32, 64);
-            t += __shfl_xor(t, 32, 64);
-            if (st.cosine && mine && qs.norm[qi] == 0.0) { // no cosine: no row is there
-                m = top[0][0] = top[0][1] = top[1][0] = top[1][1] = neg_inf();
-                s = t = 0.0f;
-            }
-            if (mine) {
-                const size_t piece = (size_t)qi * st.n_pieces + rb;
-                if (h == 0u)
-                    out.pieces[piece] = make_float4(m, s, t, 0.0f);
-                float2 *g = (float2 *)(out.groups + piece * kGroupsPerPiece); // groups 4 mt + 2 h, + 1
-                g[h] = make_float2(top[0][0], top[0][1]);
-                g[2u + h] = make_float2(top[1][0], top[1][1]);
-            }
+            for (uint32_t p = 0; p + 1u < PF; ++p)
+                ahead[p] = ahead[p + 1u];
+            ahead[PF - 1u] = first;
         }
-    } else {
-        using T = typename std::conditional<EPI == kScoresF32, float, __bf16>::type;
-        {
-            const uint32_t my = rb * 64u + lane;
+
+        // ---- epilogue: lane = query (column) r32 of tile nt; acc[mt][nt][i] = row 32 mt + 16 h + i of the row-block -------------------------
+        const Tile tile = tile_at(item);
+        const uint32_t rb = tile.rt * WAVES + wave, q0 = tile.qt * (32u * NT) + r32;
+        const bool active = rb < n_rb;
+        const uint32_t my = rb * 64u + lane; // one row per lane
+        if constexpr (EPI == kPieces) {
+            // Who is there.  Row-blocks with rows that are not there, or with a bias so low that its logit leaves the range of the exponent
+            // below, take the longer way (`masked`).
+            bool gone = my >= st.n_rows, low = false;
+            float my_mul = 1.0f, my_add = 0.0f;
+            if (!gone) {
+                my_add = st.bias ? st.bias[my] : 0.0f;
+                my_mul = st.cosine ? st.row_inv[my] : 1.0f;
+                gone = my_add == neg_inf() || (st.cosine && my_mul < 0.0f);
+                low = fabsf(my_add) > 1e30f;
+                if (SRC == kProbF32) // / 2^a
+                    my_mul *= __uint_as_float((254u << 23) - __float_as_uint(st.row_scale[my]));
+            }
+            row_mul[wave][lane] = my_mul;
+            row_add[wave][lane] = my_add;
+            const bool masked = __any(gone || low);
+            const uint64_t gone_rows = __ballot(gone);
+            const uint32_t gone_mine = (uint32_t)((gone_rows >> (16u * h)) & 0xffffu) | (uint32_t)((gone_rows >> (32u + 16u * h)) & 0xffffu) << 16;
+#pragma unroll
+            for (uint32_t nt = 0; nt < NT; ++nt) {
+                const uint32_t qi = q0 + nt * 32u;
+                const bool mine = qi < qs.nq && active;
+                const float fac = mine ? qs.fac[qi] : 0.0f;
+                float top[2][2] = {{neg_inf(), neg_inf()}, {neg_inf(), neg_inf()}}, s = 0.0f, t = 0.0f, m;
+                auto logit = [&](uint32_t mt, uint32_t i) { // (the same address in all lanes of a half)
+                    const uint32_t at = mt * 32u + h * 16u + i;
+                    return __builtin_fmaf(acc[mt][nt][i], fac * row_mul[wave][at], row_add[wave][at]);
+                };
+                auto is_gone = [&](uint32_t mt, uint32_t i) { return (gone_mine >> (16u * mt + i)) & 1u; };
+                if (!masked) {
+#pragma unroll
+                    for (uint32_t mt = 0; mt < 2u; ++mt)
+#pragma unroll
+                        for (uint32_t i = 0; i < 16u; ++i) {
+                            acc[mt][nt][i] = logit(mt, i);
+                            top[mt][i >> 3] = fmaxf(top[mt][i >> 3], acc[mt][nt][i]);
+                        }
+                    m = fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[1][0], top[1][1]));
+                    m = fmaxf(m, __uint_as_float(xor_lane32<32>(__float_as_uint(m))));
+                    const float base = piece_base(m);
+#pragma unroll
+                    for (uint32_t mt = 0; mt < 2u; ++mt)
+#pragma unroll
+                        for (uint32_t i = 0; i < 16u; ++i) {
+                            const float z = __builtin_fmaf(acc[mt][nt][i], kLog2e, -base), e = __builtin_amdgcn_exp2f(z);
+                            s += e;
+                            t = __builtin_fmaf(e, z, t);
+                        }
+                } else {
+#pragma unroll
+                    for (uint32_t mt = 0; mt < 2u; ++mt)
+#pragma unroll
+                        for (uint32_t i = 0; i < 16u; ++i) {
+                            acc[mt][nt][i] = is_gone(mt, i) ? neg_inf() : logit(mt, i);
+                            top[mt][i >> 3] = fmaxf(top[mt][i >> 3], acc[mt][nt][i]);
+                        }
+                    m = fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[1][0], top[1][1]));
+                    m = fmaxf(m, __uint_as_float(xor_lane32<32>(__float_as_uint(m))));
+                    const float base = piece_base(m);
+                    const bool huge = piece_is_huge(m);
+#pragma unroll
+                    for (uint32_t mt = 0; mt < 2u; ++mt)
+#pragma unroll
+                        for (uint32_t i = 0; i < 16u; ++i) {
+                            const float l = acc[mt][nt][i];
+                            const float z = huge ? (l - m) * kLog2e : __builtin_fmaf(l, kLog2e, -base);
+                            const float e = __builtin_amdgcn_exp2f(z);
+                            // (a row there whose logit is infinite spoils the sums; a very low finite one adds nothing)
+                            s += is_gone(mt, i) ? 0.0f : (fabsf(l) < __builtin_inff() ? e : __builtin_nanf(""));
+                            t += is_gone(mt, i) || e == 0.0f ? 0.0f : e * z;
+                        }
+                }
+                s += __uint_as_float(xor_lane32<32>(__float_as_uint(s)));
+                t += __uint_as_float(xor_lane32<32>(__float_as_uint(t)));
+                if (st.cosine && mine && qs.norm[qi] == 0.0) { // no cosine: no row is there
+                    m = top[0][0] = top[0][1] = top[1][0] = top[1][1] = neg_inf();
+                    s = t = 0.0f;
+                }
+                if (mine) {
+                    const size_t piece = (size_t)qi * st.n_pieces + rb;
+                    if (h == 0u)
+                        out.pieces[piece] = make_float4(m, s, t, 0.0f);
+                    float2 *g = (float2 *)(out.groups + piece * kGroupsPerPiece); // groups 4 mt + 2 h, + 1
+                    g[h] = make_float2(top[0][0], top[0][1]);
+                    g[2u + h] = make_float2(top[1][0], top[1][1]);
+                }
+            }
+        } else {
+            using T = typename std::conditional<EPI == kScoresF32, float, __bf16>::type;
             const float inv = st.cosine && my < st.n_rows ? st.row_inv[my] : 1.0f;
             row_mul[wave][lane] = inv < 0.0f ? __builtin_nanf("") : inv;
-        }
-        const uint32_t left = st.n_rows - rb * 64u; // rows of this block
+            const uint32_t left = active ? st.n_rows - rb * 64u : 0u; // rows of this block
 #pragma unroll
-        for (uint32_t nt = 0; nt < NT; ++nt) {
-            const uint32_t qi = q0 + nt * 32u;
-            if (qi >= qs.nq)
-                continue;
-            float fac = qs.fac[qi];
-            if (st.cosine && qs.norm[qi] == 0.0)
-                fac = __builtin_nanf("");
+            for (uint32_t nt = 0; nt < NT; ++nt) {
+                const uint32_t qi = q0 + nt * 32u;
+                if (qi < qs.nq) {
+                    const float fac = st.cosine && qs.norm[qi] == 0.0 ? __builtin_nanf("") : qs.fac[qi];
 #pragma unroll
-            for (uint32_t mt = 0; mt < 2u; ++mt) {
-                const uint32_t first = mt * 32u + h * 16u;
-                T *dst = (T *)out.scores + (size_t)qi * out.ld + rb * 64u + first;
-                T v[16];
+                    for (uint32_t mt = 0; mt < 2u; ++mt) {
+                        const uint32_t first = mt * 32u + h * 16u;
+                        T *dst = (T *)out.scores + (size_t)qi * out.ld + rb * 64u + first;
+                        T v[16];
 #pragma unroll
-                for (uint32_t i = 0; i < 16u; ++i)
-                    v[i] = (T)(acc[mt][nt][i] * fac * row_mul[wave][first + i]);
-                if (out.aligned && first + 16u <= left) {
+                        for (uint32_t i = 0; i < 16u; ++i)
+                            v[i] = (T)(acc[mt][nt][i] * fac * row_mul[wave][first + i]);
+                        if (out.aligned && first + 16u <= left) {
 #pragma unroll
-                    for (uint32_t i = 0; i < sizeof(T); ++i) {
-                        u32x4 w;
-                        __builtin_memcpy(&w, (const char *)v + 16u * i, 16);
-                        __builtin_memcpy(__builtin_assume_aligned((char *)dst + 16u * i, 16), &w, 16);
+                            for (uint32_t i = 0; i < sizeof(T); ++i) {
+                                u32x4 w;
+                                __builtin_memcpy(&w, (const char *)v + 16u * i, 16);
+                                __builtin_memcpy(__builtin_assume_aligned((char *)dst + 16u * i, 16), &w, 16);
+                            }
+                        } else {
+                            for (uint32_t i = 0; i < 16u; ++i)
+                                if (first + i < left)
+                                    dst[i] = v[i];
+                        }
                     }
-                } else {
-                    for (uint32_t i = 0; i < 16u; ++i)
-                        if (first + i < left)
-                            dst[i] = v[i];
                 }
             }
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            acc[0][nt] = acc[1][nt] = f32x16{};
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // no copy into LDS may outlive the workgroup
 }
 
-template <int SRC, int NT, int EPI>
-hipError_t run(const ProbStore &st, const ProbQueries &q, const StreamOut &out, hipStream_t s)
+template <int SRC, int NT, int WAVES, int EPI>
+hipError_t run(const ProbStore &st, const ProbQueries &q, const StreamOut &out, uint32_t n_cus, hipStream_t s)
 {
-    constexpr uint32_t kWaves = 4;
-    const uint32_t n_rb = (st.n_rows + 63u) / 64u, n_rowtiles = (n_rb + kWaves - 1u) / kWaves, n_qtiles = (q.nq + 32u * NT - 1u) / (32u * NT);
-    const uint32_t q_group = n_qtiles < 8u ? n_qtiles : 8u;
-    const uint64_t per_xcd = (uint64_t)((n_rowtiles + 7u) / 8u) * ((n_qtiles + q_group - 1u) / q_group) * q_group;
-    if (per_xcd * 8u > 0x7fffffffull)
+    const uint32_t rows = WAVES * 64u, n_rowtiles = (st.n_rows + rows - 1u) / rows, n_qtiles = (q.nq + 32u * NT - 1u) / (32u * NT);
+    const uint64_t tiles = (uint64_t)((n_rowtiles + 7u) / 8u) * n_qtiles; // of one XCD
+    if (tiles > 0x1fffffffull)
         return hipErrorInvalidValue;
-    stream_kernel<SRC, NT, kWaves, EPI><<<(uint32_t)(per_xcd * 8u), kWaves * 64u, 0, s>>>(st, q, out, n_rowtiles, n_qtiles, q_group);
+    // as many workgroups as stay resident (in even shares fewer would do, but in a last, partly filled round each is faster)
+    const uint32_t fit = (n_cus + 7u) / 8u * Step<SRC, NT, WAVES>::kWgPerCu, places = tiles < fit ? (uint32_t)tiles : fit;
+    stream_kernel<SRC, NT, WAVES, EPI><<<places * 8u, WAVES * 64u, 0, s>>>(st, q, out, n_rowtiles, n_qtiles);
     return hipGetLastError();
 }
 
 template <int SRC, int EPI>
-hipError_t run_for(const ProbStore &st, const ProbQueries &q, const StreamOut &out, hipStream_t s)
+hipError_t run_for(const ProbStore &st, const ProbQueries &q, const StreamOut &out, uint32_t n_cus, hipStream_t s)
 {
-    if (q.nq <= 32u)
-        return run<SRC, 1, EPI>(st, q, out, s);
+    // Not even one workgroup per CU: smaller ones, with longer K-steps (fewer barriers, fewer instructions between the products).
+    // 32749 rows of 777, 37 queries: 31 us of 43 (f32), 18 of 22 (f8); 100000 rows of 128, 64 queries (391 workgroups): 21 us of 15.
+    if ((uint64_t)((st.n_rows + 255u) / 256u) * ((q.nq + 63u) / 64u) < n_cus)
+        return run<SRC, 2, 2, EPI>(st, q, out, n_cus, s);
     if (q.nq <= 64u)
-        return run<SRC, 2, EPI>(st, q, out, s);
-    return run<SRC, 4, EPI>(st, q, out, s);
+        return run<SRC, 2, 4, EPI>(st, q, out, n_cus, s);
+    return run<SRC, 4, 4, EPI>(st, q, out, n_cus, s);
 }
 
 } // namespace
 
-hipError_t launch_prob_pieces(const ProbStore &st, const ProbQueries &q, float4 *pieces, float *groups, hipStream_t s)
+hipError_t launch_prob_pieces(const ProbStore &st, const ProbQueries &q, float4 *pieces, float *groups, uint32_t n_cus, hipStream_t s)
 {
     if (!st.n_pieces)
         return hipSuccess;
     const StreamOut out{pieces, groups, nullptr, 0, 0};
     if (st.source == kProbI8)
-        return run_for<kProbI8, kPieces>(st, q, out, s);
+        return run_for<kProbI8, kPieces>(st, q, out, n_cus, s);
     if (st.source == kProbF8)
-        return run_for<kProbF8, kPieces>(st, q, out, s);
-    return run_for<kProbF32, kPieces>(st, q, out, s);
+        return run_for<kProbF8, kPieces>(st, q, out, n_cus, s);
+    return run_for<kProbF32, kPieces>(st, q, out, n_cus, s);
 }
 
-hipError_t launch_f8_scores(const ProbStore &st, const ProbQueries &q, void *scores, uint64_t ld, int bf16, hipStream_t s)
+hipError_t launch_f8_scores(const ProbStore &st, const ProbQueries &q, void *scores, uint64_t ld, int bf16, uint32_t n_cus, hipStream_t s)
 {
     const uint32_t elem = bf16 ? 2u : 4u;
     const StreamOut out{nullptr, nullptr, scores, ld, ((uintptr_t)scores % 16u == 0 && ld * elem % 16u == 0) ? 1 : 0};
-    return bf16 ? run_for<kF8Raw, kScoresBf16>(st, q, out, s) : run_for<kProbF8, kScoresF32>(st, q, out, s);
+    return bf16 ? run_for<kF8Raw, kScoresBf16>(st, q, out, n_cus, s) : run_for<kProbF8, kScoresF32>(st, q, out, n_cus, s);
 }
 
 } // namespace vfsx
