@@ -397,7 +397,7 @@ struct vfsx_corpus {
     uint32_t small_off = 0;                                  // ... and how many such queries still skip it
 
     // probabilities over the store and the 8-bit floating point copy (vfsx_prob.hip, vfsx_f8.hip)
-    VmArray va_row_inv, va_row_scale, va_f8, va_f8_exp; // per row: 1 / |x|; scale of its f16 pairs; e4m3 chunks; scales
+    VmArray va_row_norm, va_row_inv, va_row_scale, va_f8, va_f8_exp; // per row: |x|; 1 / |x|; scale of its f16 pairs; e4m3 chunks; scales
     float *d_max_norm = nullptr;          // largest finite |x| of the first prob_rows rows
     uint64_t prob_rows = 0, f8_rows = 0;  // rows that the arrays cover
     bool f8_enabled = false;
@@ -1492,6 +1492,7 @@ void vfsx_corpus_destroy(vfsx_corpus *c)
     c->row_out.release();
     c->prob_work.release();
     c->prob_io.release();
+    c->va_row_norm.release();
     c->va_row_inv.release();
     c->va_row_scale.release();
     c->va_f8.release();
@@ -1610,7 +1611,7 @@ int vfsx_corpus_storage_info(vfsx_corpus *c, uint64_t *capacity_rows, uint64_t *
     return guarded([&] {
         ready(c);
         const VmArray *all[] = {&c->va_corpus, &c->va_norms, &c->va_ids, &c->va_mirror, &c->va_rn2, &c->va_inv,
-                                &c->va_row_inv, &c->va_row_scale, &c->va_f8, &c->va_f8_exp};
+                                &c->va_row_norm, &c->va_row_inv, &c->va_row_scale, &c->va_f8, &c->va_f8_exp};
         uint64_t copied = 0, bytes = 0;
         for (const VmArray *a : all) {
             copied += a->copy_bytes;
@@ -1963,6 +1964,7 @@ void fill_prob_store(vfsx_corpus *c, int source, vfsx::ProbStore &st)
     st.rows = c->d_corpus;
     st.f8 = (const uint4 *)c->va_f8.base;
     st.f8_exp = (const uint32_t *)c->va_f8_exp.base;
+    st.row_norm = (const double *)c->va_row_norm.base;
     st.row_inv = (const float *)c->va_row_inv.base;
     st.row_scale = (const float *)c->va_row_scale.base;
     st.max_norm = c->d_max_norm;
@@ -1986,9 +1988,11 @@ void ensure_prob_rows(vfsx_corpus *c, bool f8, bool capturing, hipStream_t s)
     const uint64_t pad = prob_pad(std::max<uint64_t>(c->n_rows, 1));
     if (rows_stale) {
         if (!c->va_row_inv.base && c->va_corpus.reserved) {
+            c->va_row_norm.init(c->device, max_pad * sizeof(double));
             c->va_row_inv.init(c->device, max_pad * sizeof(float));
             c->va_row_scale.init(c->device, max_pad * sizeof(float));
         }
+        c->va_row_norm.grow(pad * sizeof(double), c->prob_rows * sizeof(double), s);
         c->va_row_inv.grow(pad * sizeof(float), c->prob_rows * sizeof(float), s);
         if (c->dtype == VFSX_F32)
             c->va_row_scale.grow(pad * sizeof(float), c->prob_rows * sizeof(float), s);
@@ -1998,7 +2002,7 @@ void ensure_prob_rows(vfsx_corpus *c, bool f8, bool capturing, hipStream_t s)
         }
         vfsx::ProbStore st{};
         fill_prob_store(c, VFSX_SOURCE_ROWS, st);
-        HIP_CHECK(vfsx::launch_prob_rows(st, (uint32_t)c->prob_rows, (float *)c->va_row_inv.base,
+        HIP_CHECK(vfsx::launch_prob_rows(st, (uint32_t)c->prob_rows, (double *)c->va_row_norm.base, (float *)c->va_row_inv.base,
                                          (float *)c->va_row_scale.base, c->d_max_norm, s));
         c->prob_rows = c->n_rows;
     }
@@ -2093,9 +2097,11 @@ bool prepare_queries(const vfsx::ProbStore &st, const ProbCarve &w, char *base, 
     }
     qs.operand_chunk = 64;
     const uint32_t pad = vfsx::stream_query_pad(nq);
-    HIP_CHECK(vfsx::launch_prob_queries(st, d_queries, nq, pad, qs.fac_out, qs.eps_out, qs.norm_out, f8 ? nullptr : qs.operand_out, s));
     if (f8)
-        HIP_CHECK(vfsx::launch_f8_queries(d_queries, nq, st.dim, pad, qs.operand_out, (uint32_t *)(base + w.q8_exp), raw, s));
+        HIP_CHECK(vfsx::launch_f8_queries(st, d_queries, nq, pad, qs.fac_out, qs.eps_out, qs.norm_out, qs.operand_out,
+                                          (uint32_t *)(base + w.q8_exp), raw, s));
+    else
+        HIP_CHECK(vfsx::launch_prob_queries(st, d_queries, nq, pad, qs.fac_out, qs.eps_out, qs.norm_out, qs.operand_out, s));
     return false;
 }
 

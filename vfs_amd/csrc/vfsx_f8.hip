@@ -70,27 +70,32 @@ __global__ __launch_bounds__(64) void f8_rows_kernel(const uint4 *__restrict__ r
 }
 
 // Queries, row-major f32 -> the operand of the product: e4m3 bytes in the layout of the rows, with their scales (raw), or the same values in
-// bf16 (8 significant bits and the exponent range of f32 hold them exactly).  One wave per (query, four blocks), two elements of a block
-// per lane; queries beyond nq become zeros (the product computes whole tiles of queries).
+// bf16 (8 significant bits and the exponent range of f32 hold them exactly); and their norms and factors.  One workgroup per query, one block at
+// a time per wave, two elements per lane; queries beyond nq become zeros (the product computes whole tiles of queries).
 template <bool RAW>
-__global__ __launch_bounds__(64) void f8_queries_kernel(const float *__restrict__ q, uint32_t nq, uint32_t dim, uint32_t blocks,
-                                                        uint32_t words, uint4 *__restrict__ operand, uint32_t *__restrict__ q8_exp)
+__global__ __launch_bounds__(256) void f8_queries_kernel(ProbStore st, const float *__restrict__ q, uint32_t nq, float *__restrict__ fac,
+                                                         float *__restrict__ eps, double *__restrict__ norm,
+                                                         uint4 *__restrict__ operand, uint8_t *__restrict__ q8_exp)
 {
-    const uint32_t lane = threadIdx.x, qi = blockIdx.x, word = blockIdx.y;
+    __shared__ double squares[4];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, qi = blockIdx.x, dim = st.dim, blocks = st.f8_chunks / kF8ChunksPerBlock;
     const float *src = q + (size_t)qi * dim;
     // element k of a query lies in byte (value) k % 16 (8) of its chunk k / 16 (8); chunks are 1 KiB apart
     constexpr uint32_t kPerChunk = RAW ? 16u : 8u;
     uint8_t *dst = (uint8_t *)(operand + (size_t)(qi / 64u) * (blocks * kF8Block / kPerChunk) * 64u + (qi & 63u));
-    uint32_t exps = 0;
-    for (uint32_t j = 0; j < 4u; ++j) {
-        const uint32_t kb = word * 4u + j, k = kb * kF8Block + 2u * lane;
+    uint8_t *exp_of = q8_exp + ((size_t)(qi / 64u) * st.f8_words * 64u + (qi & 63u)) * 4u; // byte kb % 4 of dword kb / 4, those 256 bytes apart
+    double s = 0.0;
+    for (uint32_t kb = wave; kb < st.f8_words * 4u; kb += 4u) {
+        const uint32_t k = kb * kF8Block + 2u * lane;
         const float a = qi < nq && k < dim ? src[k] : 0.0f, b = qi < nq && k + 1u < dim ? src[k + 1u] : 0.0f;
+        s = __builtin_fma((double)a, (double)a, s);
+        s = __builtin_fma((double)b, (double)b, s);
         float top = fmaxf(fabsf(a), fabsf(b));
         const bool bad = __any(!(fabsf(a) < __builtin_inff()) || !(fabsf(b) < __builtin_inff()));
-        for (int o = 32; o; o >>= 1)
-            top = fmaxf(top, __shfl_xor(top, o, 64));
+        top = wave_max(top);
         const int e = bad ? 0 : f8_exponent(top);
-        exps |= (uint32_t)(e + 127) << (8u * j);
+        if (RAW && lane == 0)
+            exp_of[kb / 4u * 256u + kb % 4u] = (uint8_t)(e + 127);
         if (kb >= blocks)
             continue;
         const float by = pow2_neg(e);
@@ -103,8 +108,16 @@ __global__ __launch_bounds__(64) void f8_queries_kernel(const float *__restrict_
             *(uint32_t *)(dst + (size_t)(k / 8u) * 1024u + (k & 7u) * 2u) = __builtin_bit_cast(uint32_t, v);
         }
     }
-    if (RAW && lane == 0)
-        q8_exp[((size_t)(qi / 64u) * words + word) * 64u + (qi & 63u)] = exps;
+    s = wave_sum(s);
+    if (lane == 0)
+        squares[wave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0 && qi < nq) {
+        const QueryFactors f = query_factors(st, squares[0] + squares[1] + squares[2] + squares[3], 1.0);
+        norm[qi] = f.norm;
+        fac[qi] = f.fac;
+        eps[qi] = f.eps;
+    }
 }
 
 __global__ void f8_get_rows_kernel(const uint4 *__restrict__ f8, const uint32_t *__restrict__ f8_exp, uint32_t dim, uint32_t chunks8,
@@ -132,13 +145,13 @@ hipError_t launch_f8_rows(const uint4 *rows, uint32_t d_chunks, uint32_t dim, ui
     return hipGetLastError();
 }
 
-hipError_t launch_f8_queries(const float *q, uint32_t nq, uint32_t dim, uint32_t nq_pad, uint4 *operand, uint32_t *q8_exp, bool raw, hipStream_t s)
+hipError_t launch_f8_queries(const ProbStore &st, const float *q, uint32_t nq, uint32_t nq_pad, float *fac, float *eps, double *norm, uint4 *operand,
+                             uint32_t *q8_exp, bool raw, hipStream_t s)
 {
-    const dim3 grid(nq_pad, f8_exp_words(dim));
     if (raw)
-        f8_queries_kernel<true><<<grid, 64, 0, s>>>(q, nq, dim, f8_blocks(dim), f8_exp_words(dim), operand, q8_exp);
+        f8_queries_kernel<true><<<nq_pad, 256, 0, s>>>(st, q, nq, fac, eps, norm, operand, (uint8_t *)q8_exp);
     else
-        f8_queries_kernel<false><<<grid, 64, 0, s>>>(q, nq, dim, f8_blocks(dim), f8_exp_words(dim), operand, q8_exp);
+        f8_queries_kernel<false><<<nq_pad, 256, 0, s>>>(st, q, nq, fac, eps, norm, operand, (uint8_t *)q8_exp);
     return hipGetLastError();
 }
 

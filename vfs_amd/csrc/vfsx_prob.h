@@ -41,6 +41,7 @@ struct ProbStore {
     const uint4 *rows;     // rb64: f32 or int8
     const uint4 *f8;       // rb64: e4m3 (source f8)
     const uint32_t *f8_exp;
+    const double *row_norm; // [whole row-blocks] |x|
     const float *row_inv;  // [whole row-blocks] 1 / |x|; < 0: the row has no cosine
     const float *row_scale; // [whole row-blocks] f32 rows: 2^a with |x| 2^a <= 2^10, about
     const float *max_norm; // device scalar: the largest finite |x| of the store
@@ -50,7 +51,7 @@ struct ProbStore {
     double divide;         // what a product is divided by before the norms: T, times the int8 scale for a dot product
 };
 
-// the queries of one launch, prepared (prob_query_kernel)
+// the queries of one launch, prepared (launch_prob_queries, launch_f8_queries)
 struct ProbQueries {
     const float *q;        // [nq][dim] as the caller gave them
     const uint4 *operand;  // whole blocks of 64 queries, 16-byte chunks as in rb64: f16 pairs (f32 and int8 rows), bf16 (f8), e4m3 (f8 raw)
@@ -89,8 +90,8 @@ struct ProbFinish {
     uint32_t n_units;
 };
 
-hipError_t launch_prob_rows(const ProbStore &st, uint32_t row0, float *row_inv, float *row_scale, float *max_norm, hipStream_t s);
-// nq_pad: whole tiles of queries; those beyond nq become zeros.  `pairs` nullptr: only the factors (source f8)
+hipError_t launch_prob_rows(const ProbStore &st, uint32_t row0, double *row_norm, float *row_inv, float *row_scale, float *max_norm, hipStream_t s);
+// nq_pad: whole tiles of queries; those beyond nq become zeros
 hipError_t launch_prob_queries(const ProbStore &st, const float *q, uint32_t nq, uint32_t nq_pad, float *fac, float *eps, double *norm,
                                uint4 *pairs, hipStream_t s);
 hipError_t launch_prob_finish(const ProbStore &st, const ProbQueries &q, const ProbFinish &f, hipStream_t s);
@@ -123,7 +124,8 @@ hipError_t launch_few_scores(const ProbStore &st, const ProbQueries &q, void *ou
 hipError_t launch_f8_rows(const uint4 *rows, uint32_t d_chunks, uint32_t dim, uint32_t row0, uint32_t n_rows, uint32_t n_pad,
                           uint4 *f8, uint32_t *f8_exp, hipStream_t s);
 // raw: e4m3 bytes and scales; otherwise the same values as bf16 (exact), no scales
-hipError_t launch_f8_queries(const float *q, uint32_t nq, uint32_t dim, uint32_t nq_pad, uint4 *operand, uint32_t *q8_exp, bool raw, hipStream_t s);
+hipError_t launch_f8_queries(const ProbStore &st, const float *q, uint32_t nq, uint32_t nq_pad, float *fac, float *eps, double *norm, uint4 *operand,
+                             uint32_t *q8_exp, bool raw, hipStream_t s);
 hipError_t launch_f8_get_rows(const uint4 *f8, const uint32_t *f8_exp, uint32_t dim, const uint64_t *d_rows, uint64_t n, float *out,
                               hipStream_t s);
 

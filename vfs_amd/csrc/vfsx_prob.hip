@@ -32,12 +32,12 @@ namespace vfsx {
 
 namespace {
 
-// ---- operands of a store: 1 / |x| per row, the largest |x| -------------------------------------------------------------------
+// ---- operands of a store: |x| and 1 / |x| per row, the largest |x| -------------------------------------------------------------------
 // One thread per row.  Norms in f64: they divide every logit.  A norm whose square is zero in f32 counts as zero.
 template <int SRC>
 __global__ __launch_bounds__(256) void prob_rows_kernel(const uint4 *__restrict__ rows, uint32_t d_chunks, uint32_t row0, uint32_t n_rows,
-                                                        float *__restrict__ row_inv, float *__restrict__ row_scale,
-                                                        float *__restrict__ max_norm)
+                                                        double *__restrict__ row_norm, float *__restrict__ row_inv,
+                                                        float *__restrict__ row_scale, float *__restrict__ max_norm)
 {
     const uint64_t row = (uint64_t)row0 + (uint64_t)blockIdx.x * 256u + threadIdx.x;
     float norm = 0.0f;
@@ -47,6 +47,7 @@ __global__ __launch_bounds__(256) void prob_rows_kernel(const uint4 *__restrict_
         for (uint32_t c = 0; c < d_chunks; ++c)
             s += chunk_square<SRC>(p[(size_t)c * 64u]);
         const double r = __builtin_sqrt(s);
+        row_norm[row] = r;
         row_inv[row] = (float)s == 0.0f ? -1.0f : (float)(1.0 / r);
         if (SRC == kProbF32)
             row_scale[row] = pair_scale(r);
@@ -60,51 +61,60 @@ __global__ __launch_bounds__(256) void prob_rows_kernel(const uint4 *__restrict_
 }
 
 // ---- queries -------------------------------------------------------------------------------------------------------------------
-// One wave per query: its norm, its factor (logit = product * factor [/ |x|] + bias) and its f16 pairs.  Pairs lie as the rows do in rb64:
-// 64-query blocks of 1 KiB pieces, piece 2 c + part = elements 8 c .. 8 c + 7 of 64 queries, part 0 = hi, 1 = lo.
-__global__ __launch_bounds__(64) void prob_queries_kernel(ProbStore st, const float *__restrict__ q, uint32_t nq, uint32_t pair_chunks,
-                                                          float *__restrict__ fac, float *__restrict__ eps, double *__restrict__ norm,
-                                                          uint4 *__restrict__ pairs)
+// Eight queries per workgroup: their norms, their factors (logit = product * factor [/ |x|] + bias) and their f16 pairs.  Pairs lie as the rows do
+// in rb64: 64-query blocks of 1 KiB pieces, piece 2 c + part = elements 8 c .. 8 c + 7 of 64 queries, part 0 = hi, 1 = lo; eight
+// neighbours write 128 bytes side by side.
+constexpr uint32_t kPrepQueries = 8;
+__global__ __launch_bounds__(256) void prob_queries_kernel(ProbStore st, const float *__restrict__ q, uint32_t nq, uint32_t pair_chunks,
+                                                           float *__restrict__ fac, float *__restrict__ eps, double *__restrict__ norm,
+                                                           uint4 *__restrict__ pairs)
 {
-    const uint32_t qi = blockIdx.x, lane = threadIdx.x;
+    __shared__ float scale_of[kPrepQueries];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, q0 = blockIdx.x * kPrepQueries;
+#pragma unroll
+    for (uint32_t i = 0; i < 2u; ++i) {
+        const uint32_t qi = q0 + wave * 2u + i;
+        double s = 0.0;
+        if (qi < nq) {
+            const float *src = q + (size_t)qi * st.dim;
+#pragma unroll 4
+            for (uint32_t j = lane; j < st.dim; j += 64u) {
+                const double v = src[j];
+                s = __builtin_fma(v, v, s);
+            }
+        }
+        s = wave_sum(s);
+        const float scale = pair_scale(__builtin_sqrt(s));
+        if (lane == 0) {
+            scale_of[wave * 2u + i] = scale;
+            if (qi < nq) {
+                const QueryFactors f = query_factors(st, s, (double)scale);
+                norm[qi] = f.norm;
+                fac[qi] = f.fac;
+                eps[qi] = f.eps;
+            }
+        }
+    }
+    __syncthreads();
+    const uint32_t qi = q0 + threadIdx.x % kPrepQueries;
     const bool there = qi < nq;
     const float *src = q + (size_t)qi * st.dim;
-    double s = 0.0;
-    if (there) {
-        for (uint32_t j = lane; j < st.dim; j += 64u) {
-            const double v = src[j];
-            s = __builtin_fma(v, v, s);
-        }
-        for (int o = 32; o; o >>= 1)
-            s += __shfl_xor(s, o, 64);
-    }
-    const double r = __builtin_sqrt(s);
-    const float scale = pair_scale(r);
-    if (pairs) {
-        uint4 *dst = pairs + (size_t)(qi / 64u) * pair_chunks * 128u + (qi & 63u);
-        for (uint32_t c = lane; c < pair_chunks; c += 64u) {
-            uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-            if (there) {
+    const float scale = scale_of[threadIdx.x % kPrepQueries];
+    uint4 *dst = pairs + (size_t)(qi / 64u) * pair_chunks * 128u + (qi & 63u);
+    for (uint32_t c = threadIdx.x / kPrepQueries; c < pair_chunks; c += 256u / kPrepQueries) {
+        uint32_t hi[4], lo[4];
 #pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i) {
-                    const uint32_t k = c * 8u + i;
-                    const float x = k < st.dim ? src[k] * scale : 0.0f;
-                    const _Float16 h = (_Float16)x;
-                    const _Float16 l = (_Float16)(x - (float)h);
-                    hi[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, h) << (16u * (i & 1u));
-                    lo[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, l) << (16u * (i & 1u));
-                }
-            }
-            dst[(size_t)c * 128u] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            dst[(size_t)c * 128u + 64u] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        for (uint32_t i = 0; i < 4u; ++i) {
+            const uint32_t k = c * 8u + 2u * i;
+            const f32x2 x = {there && k < st.dim ? src[k] * scale : 0.0f, there && k + 1u < st.dim ? src[k + 1u] * scale : 0.0f};
+            const f16x2 h = __builtin_convertvector(x, f16x2);
+            const f32x2 rest = {x[0] - (float)h[0], x[1] - (float)h[1]};
+            hi[i] = __builtin_bit_cast(uint32_t, h);
+            lo[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, f16x2));
         }
+        dst[(size_t)c * 128u] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        dst[(size_t)c * 128u + 64u] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
-    if (lane || !there)
-        return;
-    const QueryFactors f = query_factors(st, s, pairs ? (double)scale : 1.0);
-    norm[qi] = f.norm;
-    fac[qi] = f.fac;
-    eps[qi] = f.eps;
 }
 
 // ---- second pass -----------------------------------------------------------------------------------------------------------------
@@ -122,30 +132,6 @@ struct FinCand {
     uint32_t pad;
 };
 
-template <int J>
-__device__ __forceinline__ double xor_d(double v)
-{
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    return __builtin_bit_cast(double, ((uint64_t)xor_lane32<J>((uint32_t)(b >> 32)) << 32) | xor_lane32<J>((uint32_t)b));
-}
-__device__ __forceinline__ double wave_sum(double v)
-{
-    v += xor_d<1>(v);
-    v += xor_d<2>(v);
-    v += xor_d<4>(v);
-    v += xor_d<8>(v);
-    v += xor_d<16>(v);
-    return v + xor_d<32>(v);
-}
-__device__ __forceinline__ float wave_max(float v)
-{
-    v = fmaxf(v, __uint_as_float(xor_lane32<1>(__float_as_uint(v))));
-    v = fmaxf(v, __uint_as_float(xor_lane32<2>(__float_as_uint(v))));
-    v = fmaxf(v, __uint_as_float(xor_lane32<4>(__float_as_uint(v))));
-    v = fmaxf(v, __uint_as_float(xor_lane32<8>(__float_as_uint(v))));
-    v = fmaxf(v, __uint_as_float(xor_lane32<16>(__float_as_uint(v))));
-    return fmaxf(v, __uint_as_float(xor_lane32<32>(__float_as_uint(v))));
-}
 __device__ __forceinline__ double lane_d(double v, uint32_t l)
 {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
@@ -169,10 +155,9 @@ __device__ __forceinline__ bool row_is_there(const ProbStore &st, const ProbQuer
     return row < st.n_rows && !(st.bias && st.bias[row] == neg_inf()) && !(st.cosine && (!(st.row_inv[row] >= 0.0f) || qs.norm[qi] == 0.0));
 }
 
-// q . x over chunks first, first + step, ... of one row, in f32 or f64; sq: the sum of squares too (f64, cosine)
-template <int SRC, typename T, bool SQ, int UNROLL>
-__device__ __forceinline__ T row_dot(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row, uint32_t first, uint32_t step,
-                                     double &sq)
+// q . x over chunks first, first + step, ... of one row, in f32 or f64
+template <int SRC, typename T, int UNROLL>
+__device__ __forceinline__ T row_dot(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row, uint32_t first, uint32_t step)
 {
     T dot = 0;
     if constexpr (SRC == kProbF8) {
@@ -183,49 +168,29 @@ __device__ __forceinline__ T row_dot(const ProbStore &st, const ProbQueries &qs,
 #pragma unroll UNROLL
         for (uint32_t c = first; c < st.f8_chunks; c += step)
             dot += scaled(f8_chunk_dot<T>(x[(size_t)c * 64u], q[(size_t)c * 2u * qc], q[((size_t)c * 2u + 1u) * qc]), f8_exp_of(xe, c / kF8ChunksPerBlock));
-    }
-    if constexpr (SRC != kProbF8 || SQ) {
-        if (SRC != kProbF8 || st.cosine) {
-            const uint4 *p = st.rows + (size_t)(row >> 6) * st.d_chunks * 64u + (row & 63u);
-            const float *q = qs.q + (size_t)qi * st.dim;
-            constexpr uint32_t per = SRC == kProbI8 ? 16u : 4u;
-            const uint32_t full = st.dim / per; // chunks without padding
+    } else {
+        const uint4 *p = st.rows + (size_t)(row >> 6) * st.d_chunks * 64u + (row & 63u);
+        const float *q = qs.q + (size_t)qi * st.dim;
+        constexpr uint32_t per = SRC == kProbI8 ? 16u : 4u;
+        const uint32_t full = st.dim / per; // chunks without padding
 #pragma unroll UNROLL
-            for (uint32_t c = first; c < full; c += step) {
-                const uint4 v = p[(size_t)c * 64u];
-                if constexpr (SRC != kProbF8)
-                    dot = chunk_dot<SRC, T>(v, q + (size_t)c * per, dot);
-                if constexpr (SQ)
-                    sq += chunk_square<SRC>(v);
-            }
-            if (full < st.d_chunks && full % step == first) {
-                const uint4 v = p[(size_t)full * 64u];
-                if constexpr (SRC != kProbF8)
-                    dot = chunk_dot_part<SRC, T>(v, q, full, st.dim, dot);
-                if constexpr (SQ)
-                    sq += chunk_square<SRC>(v);
-            }
-        }
+        for (uint32_t c = first; c < full; c += step)
+            dot = chunk_dot<SRC, T>(p[(size_t)c * 64u], q + (size_t)c * per, dot);
+        if (full < st.d_chunks && full % step == first)
+            dot = chunk_dot_part<SRC, T>(p[(size_t)full * 64u], q, full, st.dim, dot);
     }
     return dot;
 }
 
-__device__ __forceinline__ double logit_of(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row, double dot, double sq)
-{
-    return (st.cosine ? dot / (qs.norm[qi] * __builtin_sqrt(sq) * st.divide) : dot / st.divide) + (double)(st.bias ? st.bias[row] : 0.0f);
-}
-
-// the logit of one row in f64, by a whole wave
+// the logit of one row in f64, by a whole wave.  (Its norm is one of the store's: summed here, an f8 copy's would come from the f32 row, whose
+// chunks are a cache line each: 184 of the 310 MB that 512 queries of 1024 elements read.)
 template <int SRC>
 __device__ __forceinline__ double row_logit(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row)
 {
     if (!row_is_there(st, qs, qi, row)) // (uniform)
         return -__builtin_inf();
-    double sq = 0.0, dot = row_dot<SRC, double, true, 4>(st, qs, qi, row, threadIdx.x & 63u, 64u, sq);
-    dot = wave_sum(dot);
-    if (st.cosine)
-        sq = wave_sum(sq);
-    return logit_of(st, qs, qi, row, dot, sq);
+    const double dot = wave_sum(row_dot<SRC, double, 4>(st, qs, qi, row, threadIdx.x & 63u, 64u));
+    return (st.cosine ? dot / (qs.norm[qi] * st.row_norm[row] * st.divide) : dot / st.divide) + (double)(st.bias ? st.bias[row] : 0.0f);
 }
 
 // the logits of a group's 8 rows in f32 (as good as the first pass'), row lane & 7 on every lane; eighths of a wave take every eighth chunk.
@@ -236,8 +201,7 @@ __device__ __forceinline__ float group_logit(const ProbStore &st, const ProbQuer
 {
     const uint32_t lane = threadIdx.x & 63u, row = group * kGroupRows + lane % kGroupRows;
     const bool in = row_is_there(st, qs, qi, row);
-    double unused = 0.0;
-    float dot = in ? row_dot<SRC, float, false, UNROLL>(st, qs, qi, row, lane / kGroupRows, 64u / kGroupRows, unused) : 0.0f;
+    float dot = in ? row_dot<SRC, float, UNROLL>(st, qs, qi, row, lane / kGroupRows, 64u / kGroupRows) : 0.0f;
     dot += __uint_as_float(xor_lane32<8>(__float_as_uint(dot)));
     dot += __uint_as_float(xor_lane32<16>(__float_as_uint(dot)));
     dot += __uint_as_float(xor_lane32<32>(__float_as_uint(dot)));
@@ -679,15 +643,17 @@ hipError_t finish_for(const ProbStore &st, const ProbQueries &q, const ProbFinis
 
 } // namespace
 
-hipError_t launch_prob_rows(const ProbStore &st, uint32_t row0, float *row_inv, float *row_scale, float *max_norm, hipStream_t s)
+hipError_t launch_prob_rows(const ProbStore &st, uint32_t row0, double *row_norm, float *row_inv, float *row_scale, float *max_norm, hipStream_t s)
 {
     if (st.n_rows <= row0)
         return hipSuccess;
     const uint32_t blocks = (st.n_rows - row0 + 255u) / 256u;
     if (st.source == kProbI8)
-        prob_rows_kernel<kProbI8><<<blocks, 256, 0, s>>>(st.rows, st.d_chunks, row0, st.n_rows, row_inv, row_scale, max_norm);
+        prob_rows_kernel<kProbI8><<<blocks, 256, 0, s>>>(st.rows, st.d_chunks, row0, st.n_rows, row_norm, row_inv, row_scale,
+                                                                max_norm);
     else
-        prob_rows_kernel<kProbF32><<<blocks, 256, 0, s>>>(st.rows, st.d_chunks, row0, st.n_rows, row_inv, row_scale, max_norm);
+        prob_rows_kernel<kProbF32><<<blocks, 256, 0, s>>>(st.rows, st.d_chunks, row0, st.n_rows, row_norm, row_inv, row_scale,
+                                                                max_norm);
     return hipGetLastError();
 }
 
@@ -695,7 +661,7 @@ hipError_t launch_prob_queries(const ProbStore &st, const float *q, uint32_t nq,
                                uint4 *pairs, hipStream_t s)
 {
     const uint32_t chunks = query_elems(st.dim) / 8u;
-    prob_queries_kernel<<<pairs ? nq_pad : nq, 64, 0, s>>>(st, q, nq, chunks, fac, eps, norm, pairs);
+    prob_queries_kernel<<<nq_pad / kPrepQueries, 256, 0, s>>>(st, q, nq, chunks, fac, eps, norm, pairs);
     return hipGetLastError();
 }
 

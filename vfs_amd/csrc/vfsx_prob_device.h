@@ -5,6 +5,7 @@
 
 #include <type_traits>
 
+#include "vfsx_device.h"
 #include "vfsx_prob.h"
 
 namespace vfsx {
@@ -212,6 +213,31 @@ __device__ __forceinline__ float pair_scale(double r)
     e = 10 - e;
     e = e > 126 ? 126 : (e < -126 ? -126 : e);
     return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
+__device__ __forceinline__ float wave_max(float v)
+{
+    v = fmaxf(v, __uint_as_float(xor_lane32<1>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(xor_lane32<2>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(xor_lane32<4>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(xor_lane32<8>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(xor_lane32<16>(__float_as_uint(v))));
+    return fmaxf(v, __uint_as_float(xor_lane32<32>(__float_as_uint(v))));
+}
+template <int J>
+__device__ __forceinline__ double xor_d(double v)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, ((uint64_t)xor_lane32<J>((uint32_t)(b >> 32)) << 32) | xor_lane32<J>((uint32_t)b));
+}
+__device__ __forceinline__ double wave_sum(double v)
+{
+    v += xor_d<1>(v);
+    v += xor_d<2>(v);
+    v += xor_d<4>(v);
+    v += xor_d<8>(v);
+    v += xor_d<16>(v);
+    return v + xor_d<32>(v);
 }
 
 // What a query's products are multiplied by, and how far they may be off, from its sum of squares; `scale`: what its operand is scaled by.
