@@ -57,7 +57,9 @@ def score_bound(rows, q):
 
 
 SIZES = [(1, 1, 1), (2, 3, 2), (31, 16, 1), (32, 64, 3), (33, 127, 5), (64, 128, 16), (65, 129, 17), (128, 200, 33), (255, 256, 64), (257, 300, 65),
-         (1000, 96, 2), (1003, 777, 37), (5000, 130, 130), (300, 512, 300), (700, 2050, 1), (513, 1024, 257), (40000, 33, 4)]
+         (1000, 96, 2), (1003, 777, 37), (5000, 130, 130), (300, 512, 300), (700, 2050, 1), (513, 1024, 257), (40000, 33, 4),
+         # enough tiles for the large workgroups, more than one for some of them; queries too long for the kernel of a few
+         (9001, 777, 513), (30011, 72, 700), (16384, 1024, 257), (66000, 130, 33), (200003, 20, 64), (90, 5000, 8), (70, 40001, 1)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])

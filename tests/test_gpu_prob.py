@@ -72,6 +72,38 @@ def test_against_definition(store, cosine, size):
     check(corpus_of(store, rows), store, rows, q, given=given, k=k, cosine=cosine, temperature=temperature, bias=bias)
 
 
+LARGE = [  # n, d, nq: enough tiles for the large workgroups, more than one for some of them; queries too long for the first pass of a few
+    (9001, 777, 513), (30011, 72, 700), (16384, 128, 257), (66000, 130, 33), (200003, 20, 64), (300, 2100, 8), (200, 20000, 1), (70, 40001, 3),
+]
+
+
+@pytest.mark.parametrize("store", ["f32", "i8", "f8"])
+@pytest.mark.parametrize("size", LARGE, ids=lambda s: "x".join(map(str, s)))
+def test_many_tiles_and_long_rows(store, size):
+    n, d, nq = size
+    rng = np.random.default_rng(n + d)
+    rows = make(store, n, d, rng)
+    q = (2.0 * rng.standard_normal((nq, d))).astype(np.float32)
+    cosine = bool(nq % 2)
+    temperature = 0.5 / np.sqrt(d) if cosine else (0.577 * np.sqrt(d) if store == "i8" else 1.0)
+    check(corpus_of(store, rows), store, rows, q, given=rng.integers(0, n, (nq, 2)), k=7, cosine=cosine, temperature=temperature,
+          bias=masked(n, rng, ("none", "some", "lowest")[d % 3]))
+
+
+@pytest.mark.parametrize("store", ["f32", "i8", "f8"])
+@pytest.mark.parametrize("nq", [1, 40])
+def test_every_row_at_the_lowest_bias(store, nq):
+    """Logits round to the lowest f32 alike: a uniform distribution, not an empty one."""
+    rng = np.random.default_rng(21)
+    rows, q = make(store, 300, 24, rng), rng.standard_normal((nq, 24)).astype(np.float32)
+    b = np.full(300, np.finfo(np.float32).min)
+    got = corpus_of(store, rows).log_probs(q, np.array([[5, -1, 299]] * nq), 3, bias=b, source="f8" if store == "f8" else "rows")
+    assert (got.lse == b[0]).all()
+    # (f32 sums of 64 equal terms and f64 beyond are exact; what is left is the rounding of a logarithm of 300, and of what is taken from it)
+    assert np.abs(got.entropy - np.log(300)).max() <= 2.0**-17 + 2.0**-20
+    assert np.isneginf(got.log_probs[:, 1]).all() and got.top_rows.shape == (nq, 3) and (got.top_rows >= 0).all()
+
+
 @pytest.mark.parametrize("store", ["f32", "i8", "f8"])
 def test_nothing_there(store):
     rng = np.random.default_rng(1)
