@@ -61,38 +61,34 @@ __global__ __launch_bounds__(256) void prob_rows_kernel(const uint4 *__restrict_
 }
 
 // ---- queries -------------------------------------------------------------------------------------------------------------------
-// Eight queries per workgroup: their norms, their factors (logit = product * factor [/ |x|] + bias) and their f16 pairs.  Pairs lie as the rows do
-// in rb64: 64-query blocks of 1 KiB pieces, piece 2 c + part = elements 8 c .. 8 c + 7 of 64 queries, part 0 = hi, 1 = lo; eight
-// neighbours write 128 bytes side by side.
-constexpr uint32_t kPrepQueries = 8;
+// Four queries per workgroup: their norms (a wave each), their factors (logit = product * factor [/ |x|] + bias) and their f16 pairs.  Pairs lie
+// as the rows do in rb64: 64-query blocks of 1 KiB pieces, piece 2 c + part = elements 8 c .. 8 c + 7 of 64 queries, part 0 = hi, 1 = lo;
+// four neighbours write 64 bytes side by side.
+constexpr uint32_t kPrepQueries = 4;
 __global__ __launch_bounds__(256) void prob_queries_kernel(ProbStore st, const float *__restrict__ q, uint32_t nq, uint32_t pair_chunks,
                                                            float *__restrict__ fac, float *__restrict__ eps, double *__restrict__ norm,
                                                            uint4 *__restrict__ pairs)
 {
     __shared__ float scale_of[kPrepQueries];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, q0 = blockIdx.x * kPrepQueries;
-#pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i) {
-        const uint32_t qi = q0 + wave * 2u + i;
-        double s = 0.0;
-        if (qi < nq) {
-            const float *src = q + (size_t)qi * st.dim;
-#pragma unroll 4
-            for (uint32_t j = lane; j < st.dim; j += 64u) {
-                const double v = src[j];
-                s = __builtin_fma(v, v, s);
-            }
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, q0 = blockIdx.x * kPrepQueries, my = q0 + wave;
+    double s = 0.0;
+    if (my < nq) {
+        const float *src = q + (size_t)my * st.dim;
+#pragma unroll 8
+        for (uint32_t j = lane; j < st.dim; j += 64u) {
+            const double v = src[j];
+            s = __builtin_fma(v, v, s);
         }
-        s = wave_sum(s);
+    }
+    s = wave_sum(s);
+    if (lane == 0) {
         const float scale = pair_scale(__builtin_sqrt(s));
-        if (lane == 0) {
-            scale_of[wave * 2u + i] = scale;
-            if (qi < nq) {
-                const QueryFactors f = query_factors(st, s, (double)scale);
-                norm[qi] = f.norm;
-                fac[qi] = f.fac;
-                eps[qi] = f.eps;
-            }
+        scale_of[wave] = scale;
+        if (my < nq) {
+            const QueryFactors f = query_factors(st, s, (double)scale);
+            norm[my] = f.norm;
+            fac[my] = f.fac;
+            eps[my] = f.eps;
         }
     }
     __syncthreads();

@@ -39,13 +39,15 @@ namespace {
 enum { kF8Raw = 3 }; // beside ProbSource
 
 // What one K-step is: kSlotData bytes of queries, as many elements as that is for 32 NT queries.  WAVES row-blocks per workgroup: four, or
-// two where there are few tiles; then nothing but more loads on their way hides a load's latency, and there are registers for them.
-template <int SRC, int NT, int WAVES>
+// two where there are few tiles, each by QW = 2 waves with half of the queries; then nothing but more loads on their way hides a load's
+// latency, and there are registers for them.
+template <int SRC, int NT, int WAVES, int QW>
 struct Step {
+    static constexpr uint32_t kWaves = WAVES * QW, kQTiles = NT * QW;
     static constexpr uint32_t kQParts = SRC == kProbF32 || SRC == kProbI8 ? 2u : 1u; // hi, lo
     static constexpr uint32_t kQBytes = SRC == kF8Raw ? 1u : 2u;                      // of an element of a part
-    static constexpr uint32_t kSlotData = (SRC == kProbI8 ? 4096u : 2048u) * NT * (WAVES == 2 ? 2u : 1u);
-    static constexpr uint32_t kElems = kSlotData / (32u * NT * kQParts * kQBytes);
+    static constexpr uint32_t kSlotData = (SRC == kProbI8 ? 4096u : 2048u) * kQTiles * (WAVES == 2 ? 2u : 1u);
+    static constexpr uint32_t kElems = kSlotData / (32u * kQTiles * kQParts * kQBytes);
     static constexpr uint32_t kQChunks = kElems * kQBytes / 16u;
     static constexpr uint32_t kChunks = kElems / (SRC == kProbF32 ? 4u : 16u); // of a row
     static constexpr uint32_t kTileLoads = kChunks / 2u;                       // per lane and A tile: half of a row's chunks each
@@ -54,30 +56,34 @@ struct Step {
     static constexpr uint32_t kPieces = kSlotData / 1024u;                     // 1 KiB each: one copy by one wave
     static constexpr uint32_t kExpDma = SRC == kF8Raw ? 1u : 0u;               // raw: the queries' exponents
     // vector memory instructions of a wave and K-step
-    static constexpr uint32_t kDma = kPieces / WAVES + kExpDma, kA = kLoads + kRowWords;
+    static constexpr uint32_t kDma = kPieces / kWaves + kExpDma, kA = kLoads + kRowWords;
     static constexpr uint32_t kSlotBytes = kSlotData + kExpDma * 1024u;
     static constexpr uint32_t kSlots = SRC == kProbI8 ? 3u : 5u;
     static constexpr uint32_t kPf = kLoads <= 2u || (WAVES == 2 && kLoads == 4u) ? 4u : 3u;
     static constexpr uint32_t kWavesPerSimd = WAVES == 2 || NT == 4 ? 2u : 3u;
-    static constexpr uint32_t kWgPerCu = kWavesPerSimd * 4u / WAVES;
+    static constexpr uint32_t kWgPerCu = kWavesPerSimd * 4u / kWaves;
     // The queries of a K-step are here when at most this many younger instructions are on their way: the copies of the kSlots - 2 younger
     // slots and the rows' loads issued since (in the first steps those of the prologue, at least min(kPf, kSlots - 2) of them; anything
     // else that was issued since makes this stricter).
     static constexpr uint32_t kYounger = (kSlots - 2u) * kDma + (kPf < kSlots - 2u ? kPf : kSlots - 2u) * kA;
-    static_assert(kElems >= 16u && kElems <= kF8Block && kPieces % WAVES == 0 && kYounger < 64u, "a K-step");
+    static_assert(kElems >= 16u && kElems <= kF8Block && kPieces % kWaves == 0 && kYounger < 64u, "a K-step");
 };
 
-template <int SRC, int NT, int WAVES, int EPI>
-__global__ __launch_bounds__(WAVES * 64, (Step<SRC, NT, WAVES>::kWavesPerSimd)) void stream_kernel(ProbStore st, ProbQueries qs, StreamOut out,
+template <int SRC, int NT, int WAVES, int QW, int EPI>
+__global__ __launch_bounds__(WAVES * QW * 64, (Step<SRC, NT, WAVES, QW>::kWavesPerSimd)) void stream_kernel(ProbStore st, ProbQueries qs, StreamOut out,
                                                                                                   uint32_t n_rowtiles, uint32_t n_qtiles)
 {
-    using S = Step<SRC, NT, WAVES>;
+    using S = Step<SRC, NT, WAVES, QW>;
     constexpr bool kIsF8 = SRC == kProbF8 || SRC == kF8Raw;
     constexpr uint32_t kSlots = S::kSlots, PF = S::kPf;
     __shared__ __align__(1024) uint8_t ring[kSlots * S::kSlotBytes];
-    __shared__ __align__(16) float row_mul[WAVES][64], row_add[WAVES][64]; // epilogue: each wave its own rows
+    __shared__ __align__(16) float row_mul[S::kWaves][64], row_add[S::kWaves][64]; // epilogue: each wave its own rows
+    using T = typename std::conditional<EPI == kScoresBf16, __bf16, float>::type;
+    constexpr uint32_t kTurnPitch = 32u + 16u / sizeof(T); // of 32 queries by 32 scores (a multiple of 16 bytes, neighbours in other banks)
+    __shared__ __align__(16) T turn[EPI == kPieces ? 1 : S::kWaves][EPI == kPieces ? 1 : 32u * kTurnPitch];
     const uint32_t lane = threadIdx.x & 63u, h = lane >> 5, r32 = lane & 31u;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t rw = wave % WAVES, qw = wave / WAVES; // its row-block and its part of the queries
     const uint32_t perm = 16u * ((r32 >> 2) & 1u) + 4u * (r32 >> 3) + (r32 & 3u); // store row (in its tile of 32) of matrix row r32
 
     // Tiles.  Workgroups with the same id % 8 share an XCD and its L2.  An XCD owns every eighth row tile; its list goes through groups of (up
@@ -112,7 +118,7 @@ __global__ __launch_bounds__(WAVES * 64, (Step<SRC, NT, WAVES>::kWavesPerSimd)) 
     auto next_queries = [&] {
         b_step = 0;
         b_qt = tile_at(b_item++).qt;
-        b_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)qs.operand + (size_t)b_qt * (NT / 2u) * q_block_bytes), 0, 0xffffffffu,
+        b_rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)qs.operand + (size_t)b_qt * (S::kQTiles / 2u) * q_block_bytes), 0, 0xffffffffu,
                                                    0x00020000);
     };
     next_queries();
@@ -125,16 +131,16 @@ __global__ __launch_bounds__(WAVES * 64, (Step<SRC, NT, WAVES>::kWavesPerSimd)) 
     auto stage_queries = [&] {
         const uint32_t slot = lds0 + b_slot * S::kSlotBytes;
 #pragma unroll
-        for (uint32_t i = 0; i < S::kPieces / WAVES; ++i) {
-            const uint32_t piece = wave * (S::kPieces / WAVES) + i;
-            constexpr uint32_t per_tile = S::kPieces / NT;
+        for (uint32_t i = 0; i < S::kPieces / S::kWaves; ++i) {
+            const uint32_t piece = wave * (S::kPieces / S::kWaves) + i;
+            constexpr uint32_t per_tile = S::kPieces / S::kQTiles;
             const uint32_t tile32 = piece / per_tile, pair = piece % per_tile;
             dma(b_rsrc, slot + piece * 1024u, h * 1024u + r32 * 16u,
                 (tile32 >> 1) * q_block_bytes + (tile32 & 1u) * 512u + (b_step * S::kQChunks * S::kQParts + 2u * pair) * 1024u);
         }
         if (S::kExpDma) { // (every wave the same 1 KiB) a dword of exponents for each query: 16 bytes of a 64-query block per lane
             const uint32_t word = b_step * S::kElems / (4u * kF8Block);
-            const uint32_t block = min(b_qt * (NT / 2u) + (lane >> 4), (qs.nq - 1u) / 64u); // (four blocks' worth; the tile has NT / 2)
+            const uint32_t block = min(b_qt * (S::kQTiles / 2u) + (lane >> 4), (qs.nq - 1u) / 64u); // (four blocks' worth; the tile has kQTiles / 2)
             dma(e_rsrc, slot + S::kSlotData, (block * st.f8_words + word) * 256u + (lane & 15u) * 16u, 0);
         }
         if (++b_slot == kSlots)
@@ -152,7 +158,7 @@ __global__ __launch_bounds__(WAVES * 64, (Step<SRC, NT, WAVES>::kWavesPerSimd)) 
     const uint4 *a_from = nullptr;
     const uint32_t *a_words = nullptr;
     auto next_rows = [&] {
-        const uint32_t my_rb = tile_at(a_item).rt * WAVES + wave, rb = min(my_rb, n_rb - 1u);
+        const uint32_t my_rb = tile_at(a_item).rt * WAVES + rw, rb = min(my_rb, n_rb - 1u);
         a_step = 0;
         a_from = rows + (size_t)rb * row_chunks * 64u;
         a_chunk = my_rb < n_rb && a_item < my_tiles ? 1024u : 0u;
@@ -206,7 +212,7 @@ __global__ __launch_bounds__(WAVES * 64, (Step<SRC, NT, WAVES>::kWavesPerSimd)) 
         asm volatile("" ::: "memory");
         const uint8_t *q_slot = ring + slot * S::kSlotBytes;
         auto q_frag = [&](uint32_t nt, uint32_t chunk, uint32_t part) {
-            return *(const u32x4 *)(q_slot + ((nt * S::kQChunks + chunk) * S::kQParts + part) * 512u + r32 * 16u);
+            return *(const u32x4 *)(q_slot + (((qw * NT + nt) * S::kQChunks + chunk) * S::kQParts + part) * 512u + r32 * 16u);
         };
         if constexpr (SRC == kF8Raw) {
             const uint32_t sh = 8u * ((step * S::kElems / kF8Block) & 3u);
@@ -222,7 +228,7 @@ __global__ __launch_bounds__(WAVES * 64, (Step<SRC, NT, WAVES>::kWavesPerSimd)) 
                 for (uint32_t nt = 0; nt < NT; ++nt) {
                     const u32x4 p = q_frag(nt, 4u * s + 2u * h, 0), q = q_frag(nt, 4u * s + 2u * h + 1u, 0);
                     const i32x8 fb = {(int)p[0], (int)p[1], (int)p[2], (int)p[3], (int)q[0], (int)q[1], (int)q[2], (int)q[3]};
-                    const uint32_t e = *(const uint32_t *)(q_slot + S::kSlotData + (nt * 32u + r32) * 4u);
+                    const uint32_t e = *(const uint32_t *)(q_slot + S::kSlotData + ((qw * NT + nt) * 32u + r32) * 4u);
 #pragma unroll
                     for (uint32_t mt = 0; mt < 2u; ++mt)
                         acc[mt][nt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[mt], fb, acc[mt][nt], 0, 0, 0, (int)(x.word[mt] >> sh),
@@ -336,7 +342,7 @@ __global__ __launch_bounds__(WAVES * 64, (Step<SRC, NT, WAVES>::kWavesPerSimd)) 
 
         // ---- epilogue: lane = query (column) r32 of tile nt; acc[mt][nt][i] = row 32 mt + 16 h + i of the row-block -------------------------
         const Tile tile = tile_at(item);
-        const uint32_t rb = tile.rt * WAVES + wave, q0 = tile.qt * (32u * NT) + r32;
+        const uint32_t rb = tile.rt * WAVES + rw, q0 = (tile.qt * S::kQTiles + qw * NT) * 32u + r32;
         const bool active = rb < n_rb;
         const uint32_t my = rb * 64u + lane; // one row per lane
         if constexpr (EPI == kPieces) {
@@ -427,34 +433,47 @@ __global__ __launch_bounds__(WAVES * 64, (Step<SRC, NT, WAVES>::kWavesPerSimd)) 
                 }
             }
         } else {
-            using T = typename std::conditional<EPI == kScoresF32, float, __bf16>::type;
             const float inv = st.cosine && my < st.n_rows ? st.row_inv[my] : 1.0f;
             row_mul[wave][lane] = inv < 0.0f ? __builtin_nanf("") : inv;
             const uint32_t left = active ? st.n_rows - rb * 64u : 0u; // rows of this block
+            const bool whole = out.aligned && left >= 64u;
 #pragma unroll
             for (uint32_t nt = 0; nt < NT; ++nt) {
                 const uint32_t qi = q0 + nt * 32u;
-                if (qi < qs.nq) {
-                    const float fac = st.cosine && qs.norm[qi] == 0.0 ? __builtin_nanf("") : qs.fac[qi];
+                float fac = 0.0f;
+                if (qi < qs.nq)
+                    fac = st.cosine && qs.norm[qi] == 0.0 ? __builtin_nanf("") : qs.fac[qi];
 #pragma unroll
-                    for (uint32_t mt = 0; mt < 2u; ++mt) {
-                        const uint32_t first = mt * 32u + h * 16u;
-                        T *dst = (T *)out.scores + (size_t)qi * out.ld + rb * 64u + first;
-                        T v[16];
+                for (uint32_t mt = 0; mt < 2u; ++mt) {
+                    const uint32_t first = mt * 32u + h * 16u;
+                    T v[16];
 #pragma unroll
-                        for (uint32_t i = 0; i < 16u; ++i)
-                            v[i] = (T)(acc[mt][nt][i] * fac * row_mul[wave][first + i]);
-                        if (out.aligned && first + 16u <= left) {
+                    for (uint32_t i = 0; i < 16u; ++i)
+                        v[i] = (T)(acc[mt][nt][i] * fac * row_mul[wave][first + i]);
+                    if (whole) {
+                        if (qi < qs.nq) {
+                            T *dst = (T *)out.scores + (size_t)qi * out.ld + rb * 64u + first;
 #pragma unroll
                             for (uint32_t i = 0; i < sizeof(T); ++i) {
                                 u32x4 w;
                                 __builtin_memcpy(&w, (const char *)v + 16u * i, 16);
                                 __builtin_memcpy(__builtin_assume_aligned((char *)dst + 16u * i, 16), &w, 16);
                             }
-                        } else {
-                            for (uint32_t i = 0; i < 16u; ++i)
-                                if (first + i < left)
-                                    dst[i] = v[i];
+                        }
+                    } else {
+                        // Rows of the output that begin anywhere, or end here: a score at a time, but 32 neighbours of two queries by one
+                        // instruction, turned through LDS (a lane's own 16 scores: 64 lines an instruction; 37 queries, 32749 rows: 17.7 us,
+                        // turned 12.7).
+#pragma unroll
+                        for (uint32_t i = 0; i < sizeof(T); ++i)
+                            __builtin_memcpy(__builtin_assume_aligned((char *)&turn[wave][r32 * kTurnPitch + h * 16u] + 16u * i, 16),
+                                             (const char *)v + 16u * i, 16);
+#pragma unroll
+                        for (uint32_t j = 0; j < 16u; ++j) {
+                            const T one = turn[wave][(2u * j + h) * kTurnPitch + r32];
+                            const uint32_t to = q0 - r32 + nt * 32u + 2u * j + h, row = mt * 32u + r32;
+                            if (to < qs.nq && row < left)
+                                ((T *)out.scores)[(size_t)to * out.ld + rb * 64u + row] = one;
                         }
                     }
                 }
@@ -467,29 +486,32 @@ __global__ __launch_bounds__(WAVES * 64, (Step<SRC, NT, WAVES>::kWavesPerSimd)) 
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // no copy into LDS may outlive the workgroup
 }
 
-template <int SRC, int NT, int WAVES, int EPI>
+template <int SRC, int NT, int WAVES, int QW, int EPI>
 hipError_t run(const ProbStore &st, const ProbQueries &q, const StreamOut &out, uint32_t n_cus, hipStream_t s)
 {
-    const uint32_t rows = WAVES * 64u, n_rowtiles = (st.n_rows + rows - 1u) / rows, n_qtiles = (q.nq + 32u * NT - 1u) / (32u * NT);
+    using S = Step<SRC, NT, WAVES, QW>;
+    constexpr uint32_t rows = WAVES * 64u, queries = S::kQTiles * 32u;
+    const uint32_t n_rowtiles = (st.n_rows + rows - 1u) / rows, n_qtiles = (q.nq + queries - 1u) / queries;
     const uint64_t tiles = (uint64_t)((n_rowtiles + 7u) / 8u) * n_qtiles; // of one XCD
     if (tiles > 0x1fffffffull)
         return hipErrorInvalidValue;
     // as many workgroups as stay resident (in even shares fewer would do, but in a last, partly filled round each is faster)
-    const uint32_t fit = (n_cus + 7u) / 8u * Step<SRC, NT, WAVES>::kWgPerCu, places = tiles < fit ? (uint32_t)tiles : fit;
-    stream_kernel<SRC, NT, WAVES, EPI><<<places * 8u, WAVES * 64u, 0, s>>>(st, q, out, n_rowtiles, n_qtiles);
+    const uint32_t fit = (n_cus + 7u) / 8u * S::kWgPerCu, places = tiles < fit ? (uint32_t)tiles : fit;
+    stream_kernel<SRC, NT, WAVES, QW, EPI><<<places * 8u, S::kWaves * 64u, 0, s>>>(st, q, out, n_rowtiles, n_qtiles);
     return hipGetLastError();
 }
 
 template <int SRC, int EPI>
 hipError_t run_for(const ProbStore &st, const ProbQueries &q, const StreamOut &out, uint32_t n_cus, hipStream_t s)
 {
-    // Not even one workgroup per CU: smaller ones, with longer K-steps (fewer barriers, fewer instructions between the products).
-    // 32749 rows of 777, 37 queries: 31 us of 43 (f32), 18 of 22 (f8); 100000 rows of 128, 64 queries (391 workgroups): 21 us of 15.
+    // Not even one workgroup per CU: smaller ones, with longer K-steps (fewer barriers, fewer instructions between the products) and twice the
+    // waves for the same rows (half of the SIMDs would have none).  32749 rows of 777, 37 queries: 27 us of 43 (f32), 12.7 of 17.5 (f8);
+    // 100000 rows of 128, 64 queries (391 workgroups): 21 us of 15.
     if ((uint64_t)((st.n_rows + 255u) / 256u) * ((q.nq + 63u) / 64u) < n_cus)
-        return run<SRC, 2, 2, EPI>(st, q, out, n_cus, s);
+        return run<SRC, 1, 2, 2, EPI>(st, q, out, n_cus, s);
     if (q.nq <= 64u)
-        return run<SRC, 2, 4, EPI>(st, q, out, n_cus, s);
-    return run<SRC, 4, 4, EPI>(st, q, out, n_cus, s);
+        return run<SRC, 2, 4, 1, EPI>(st, q, out, n_cus, s);
+    return run<SRC, 4, 4, 1, EPI>(st, q, out, n_cus, s);
 }
 
 } // namespace
