@@ -131,28 +131,9 @@ __global__ __launch_bounds__(kFewWaves * 64, 3) void few_kernel(ProbStore st, co
     __shared__ QueryFactors factors[NQS];
     const uint32_t lane = threadIdx.x & 63u, h = lane >> 5, r32 = lane & 31u;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    for (uint32_t i = wave; i < NQS; i += kFewWaves) {
-        QueryFactors f;
-        prepare_query<SRC, NQS>(st, i < nq ? q + (size_t)i * st.dim : nullptr, i, elems, q_lds, f);
-        if (lane == 0) {
-            factors[i] = f;
-            if (blockIdx.x == 0 && i < nq) { // for the second pass
-                qs.fac_out[i] = f.fac;
-                qs.eps_out[i] = f.eps;
-                qs.norm_out[i] = f.norm;
-            }
-        }
-    }
-    __syncthreads();
-    if (SRC == kProbF8 && blockIdx.x == 0)
-        for (uint32_t i = threadIdx.x; i < elems / 8u * NQS; i += kFewWaves * 64u)
-            qs.operand_out[i] = ((const uint4 *)q_lds)[i];
-
     const uint32_t n_rb = (st.n_rows + 63u) / 64u, n_step = (st.dim + kStepElems<SRC> - 1u) / kStepElems<SRC>;
     const uint32_t first = blockIdx.x * kFewWaves + wave, stride = gridDim.x * kFewWaves;
-    if (first >= n_rb)
-        return;
-    const uint32_t my_rb = (n_rb - first + stride - 1u) / stride, total = my_rb * n_step;
+    const uint32_t my_rb = first < n_rb ? (n_rb - first + stride - 1u) / stride : 0u, total = my_rb * n_step;
     const uint32_t row_chunks = SRC == kProbF8 ? st.f8_chunks : st.d_chunks;
     const uint4 *rows = SRC == kProbF8 ? st.f8 : st.rows;
 
@@ -162,11 +143,12 @@ __global__ __launch_bounds__(kFewWaves * 64, 3) void few_kernel(ProbStore st, co
         uint32_t of_row[2]; // f32: the rows' scales; f8: their dwords of exponents
     };
     Ahead ahead[PF];
-    uint32_t p_rb = first, p_step = 0;
+    uint32_t p_rb = min(first, n_rb - 1u), p_step = 0, p_at = 0;
     auto load = [&](Ahead &x) {
-        // bounded by the row-block: chunks beyond a row's last read as zeros
+        // bounded by the row-block: chunks beyond a row's last read as zeros, and past the last block nothing is read
         const __amdgpu_buffer_rsrc_t rsrc =
-            __builtin_amdgcn_make_buffer_rsrc((void *)(rows + (size_t)p_rb * row_chunks * 64u), 0, row_chunks * 1024u, 0x00020000);
+            __builtin_amdgcn_make_buffer_rsrc((void *)(rows + (size_t)p_rb * row_chunks * 64u), 0, p_at < total ? row_chunks * 1024u : 0u, 0x00020000);
+        ++p_at;
 #pragma unroll
         for (uint32_t i = 0; i < 8u; ++i) {
             const uint32_t tile = i >> 2, j = i & 3u;
@@ -188,6 +170,27 @@ __global__ __launch_bounds__(kFewWaves * 64, 3) void few_kernel(ProbStore st, co
 #pragma unroll
     for (uint32_t p = 0; p < PF; ++p)
         load(ahead[p]);
+
+    // ---- queries, while the first rows are on their way --------------------------------------------------------------------------------
+    for (uint32_t i = wave; i < NQS; i += kFewWaves) {
+        QueryFactors f;
+        prepare_query<SRC, NQS>(st, i < nq ? q + (size_t)i * st.dim : nullptr, i, elems, q_lds, f);
+        if (lane == 0) {
+            factors[i] = f;
+            if (blockIdx.x == 0 && i < nq) { // for the second pass
+                qs.fac_out[i] = f.fac;
+                qs.eps_out[i] = f.eps;
+                qs.norm_out[i] = f.norm;
+            }
+        }
+    }
+    __syncthreads();
+    if (SRC == kProbF8 && blockIdx.x == 0)
+        for (uint32_t i = threadIdx.x; i < elems / 8u * NQS; i += kFewWaves * 64u)
+            qs.operand_out[i] = ((const uint4 *)q_lds)[i];
+
+    if (!my_rb)
+        return;
 
     // ---- epilogue of a row-block -------------------------------------------------------------------------------------------------------
     using Acc = typename std::conditional<SRC == kProbI8, i32x16, f32x16>::type;
