@@ -138,9 +138,16 @@ __global__ __launch_bounds__(kFewWaves * 64, 3) void few_kernel(ProbStore st, co
     const uint4 *rows = SRC == kProbF8 ? st.f8 : st.rows;
 
     // ---- loads, PF K-steps ahead -----------------------------------------------------------------------------------------------------
+    // NQS <= 4: both halves of the wave hold the same products; half h goes on with tile h, one row per lane.  NQS = 8: half h holds queries
+    // 4 h .. 4 h + 3 and both tiles.
+    constexpr uint32_t TILES = NQS <= 4u ? 1u : 2u;
+    struct Tail { // what the epilogue needs of its rows, loaded with the last K-step (after the loads ahead it would wait for all of those)
+        float inv[TILES], bias[TILES];
+    };
     struct Ahead {
         u32x4 a[8];
         uint32_t of_row[2]; // f32: the rows' scales; f8: their dwords of exponents
+        Tail tail;
     };
     Ahead ahead[PF];
     uint32_t p_rb = min(first, n_rb - 1u), p_step = 0, p_at = 0;
@@ -163,6 +170,14 @@ __global__ __launch_bounds__(kFewWaves * 64, 3) void few_kernel(ProbStore st, co
                 x.of_row[tile] = st.f8_exp[((size_t)p_rb * st.f8_words + (p_step >> 2)) * 64u + tile * 32u + r32];
         }
         if (++p_step == n_step) {
+#pragma unroll
+            for (uint32_t t = 0; t < TILES; ++t) {
+                const uint32_t row = min(p_rb * 64u + (TILES == 1u ? lane : t * 32u + r32), st.n_rows - 1u);
+                if (st.cosine)
+                    x.tail.inv[t] = st.row_inv[row];
+                if (EPI == kPieces && st.bias)
+                    x.tail.bias[t] = st.bias[row];
+            }
             p_step = 0;
             p_rb = p_rb + stride < n_rb ? p_rb + stride : p_rb; // (past the end: the last one again)
         }
@@ -196,16 +211,13 @@ __global__ __launch_bounds__(kFewWaves * 64, 3) void few_kernel(ProbStore st, co
     using Acc = typename std::conditional<SRC == kProbI8, i32x16, f32x16>::type;
     Acc acc[2] = {};
     constexpr uint32_t SLOTS = NQS < 4u ? NQS : 4u;
-    // NQS <= 4: both halves of the wave hold the same products; half h goes on with tile h, one row per lane.  NQS = 8: half h holds queries
-    // 4 h .. 4 h + 3 and both tiles.
-    constexpr uint32_t TILES = NQS <= 4u ? 1u : 2u;
     auto product = [&](uint32_t tile, uint32_t b) -> float {
         if constexpr (SRC == kProbI8)
             return __builtin_fmaf((float)acc[tile][b], 65536.0f, __builtin_fmaf((float)acc[tile][4u + b], 256.0f, (float)acc[tile][8u + b]));
         else
             return acc[tile][b];
     };
-    auto finish_block = [&](uint32_t rb) __attribute__((always_inline)) {
+    auto finish_block = [&](uint32_t rb, const Tail &tail, const uint32_t *of_row) __attribute__((always_inline)) {
         float mul[TILES], add[TILES];
         bool gone[TILES];
 #pragma unroll
@@ -216,14 +228,14 @@ __global__ __launch_bounds__(kFewWaves * 64, 3) void few_kernel(ProbStore st, co
             mul[t] = 1.0f;
             if (!gone[t]) {
                 if (EPI == kPieces && st.bias)
-                    add[t] = st.bias[row];
+                    add[t] = tail.bias[t];
                 if (st.cosine)
-                    mul[t] = st.row_inv[row];
+                    mul[t] = tail.inv[t];
                 gone[t] = EPI == kPieces && (add[t] == neg_inf() || (st.cosine && mul[t] < 0.0f));
                 if (EPI != kPieces && st.cosine && mul[t] < 0.0f)
                     mul[t] = __builtin_nanf("");
                 if (SRC == kProbF32) // / 2^a
-                    mul[t] *= __uint_as_float((254u << 23) - __float_as_uint(st.row_scale[row]));
+                    mul[t] *= __uint_as_float((254u << 23) - (TILES == 1u ? (h ? of_row[1] : of_row[0]) : of_row[t]));
             }
         }
 #pragma unroll
@@ -341,9 +353,11 @@ __global__ __launch_bounds__(kFewWaves * 64, 3) void few_kernel(ProbStore st, co
                     }
                 }
             }
+            const Tail tail = x.tail;
+            const uint32_t of_row[2] = {x.of_row[0], x.of_row[1]};
             load(x);
             if (++step == n_step) {
-                finish_block(rb);
+                finish_block(rb, tail, of_row);
                 acc[0] = Acc{};
                 acc[1] = Acc{};
                 step = 0;
