@@ -18,7 +18,8 @@ Deliberate deviations (documented in DESIGN.md)
     by the exact engine -- the HNSW path is out of scope;
   * a registered vector is searchable at once and appears once (the reference returns memtable
     vectors twice); a quantizing store shows the flushed form of a vector
-    (name + "_quantized", tag "quantized", vector.rs:116-121) from the start.
+    (name + "_quantized", tag "quantized", vector.rs:116-121) from the start;
+  * `/search` takes an optional "temperature" (cosine methods): "log_prob" per hit and "entropy" beside the reference's fields.
 """
 from __future__ import annotations
 
