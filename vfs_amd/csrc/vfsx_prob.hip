@@ -121,6 +121,7 @@ constexpr uint32_t kFinGroups = 1024; // candidate groups kept at once
 constexpr uint32_t kFinRows = 1024;   // candidate rows kept at once
 constexpr uint32_t kBuckets = 256;    // maxima that the first bound of many rows is taken from
 static_assert(kBuckets >= VFSX_LOG_PROBS_MAX_K, "the first bound is one of them");
+static_assert(kFinGroups >= kFinRows && kFinGroups >= 64u * kGroupRows + VFSX_LOG_PROBS_MAX_K, "ranks of all candidates");
 
 struct FinCand {
     double l;
@@ -146,9 +147,28 @@ __device__ __forceinline__ float wave_kth(float v, const float *lds, uint32_t k)
     return -wave_max(above < k ? -v : neg_inf());
 }
 
-__device__ __forceinline__ bool row_is_there(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row)
+// what a logit has of its row beside the product; `in`: the row is there.  All loads at once, and before the product's (one after the
+// other they are waited for one by one).
+struct RowPart {
+    bool in;
+    float bias, inv;
+    double norm;
+};
+template <bool NORM>
+__device__ __forceinline__ RowPart row_part(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row)
 {
-    return row < st.n_rows && !(st.bias && st.bias[row] == neg_inf()) && !(st.cosine && (!(st.row_inv[row] >= 0.0f) || qs.norm[qi] == 0.0));
+    RowPart p{true, 0.0f, 1.0f, 1.0};
+    double q_norm = 1.0;
+    if (st.bias)
+        p.bias = st.bias[row];
+    if (st.cosine) {
+        p.inv = st.row_inv[row];
+        if (NORM)
+            p.norm = st.row_norm[row];
+        q_norm = qs.norm[qi];
+    }
+    p.in = p.bias != neg_inf() && p.inv >= 0.0f && q_norm != 0.0;
+    return p;
 }
 
 // q . x over chunks first, first + step, ... of one row, in f32 or f64
@@ -183,10 +203,9 @@ __device__ __forceinline__ T row_dot(const ProbStore &st, const ProbQueries &qs,
 template <int SRC>
 __device__ __forceinline__ double row_logit(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t row)
 {
-    if (!row_is_there(st, qs, qi, row)) // (uniform)
-        return -__builtin_inf();
+    const RowPart p = row_part<true>(st, qs, qi, row);
     const double dot = wave_sum(row_dot<SRC, double, 4>(st, qs, qi, row, threadIdx.x & 63u, 64u));
-    return (st.cosine ? dot / (qs.norm[qi] * st.row_norm[row] * st.divide) : dot / st.divide) + (double)(st.bias ? st.bias[row] : 0.0f);
+    return p.in ? (st.cosine ? dot / (qs.norm[qi] * p.norm * st.divide) : dot / st.divide) + (double)p.bias : -__builtin_inf();
 }
 
 // the logits of a group's 8 rows in f32 (as good as the first pass'), row lane & 7 on every lane; eighths of a wave take every eighth chunk.
@@ -196,33 +215,55 @@ template <int SRC, int UNROLL>
 __device__ __forceinline__ float group_logit(const ProbStore &st, const ProbQueries &qs, uint32_t qi, uint32_t group, float fac)
 {
     const uint32_t lane = threadIdx.x & 63u, row = group * kGroupRows + lane % kGroupRows;
-    const bool in = row_is_there(st, qs, qi, row);
-    float dot = in ? row_dot<SRC, float, UNROLL>(st, qs, qi, row, lane / kGroupRows, 64u / kGroupRows) : 0.0f;
+    const RowPart p = row_part<false>(st, qs, qi, min(row, st.n_rows - 1u));
+    float dot = row_dot<SRC, float, UNROLL>(st, qs, qi, min(row, st.n_rows - 1u), lane / kGroupRows, 64u / kGroupRows);
     dot += __uint_as_float(xor_lane32<8>(__float_as_uint(dot)));
     dot += __uint_as_float(xor_lane32<16>(__float_as_uint(dot)));
     dot += __uint_as_float(xor_lane32<32>(__float_as_uint(dot)));
-    if (!in)
-        return neg_inf();
-    return dot * fac * (st.cosine ? st.row_inv[row] : 1.0f) + (st.bias ? st.bias[row] : 0.0f);
+    return p.in && row < st.n_rows ? dot * fac * p.inv + p.bias : neg_inf();
 }
 __device__ __forceinline__ bool cand_before(double la, uint32_t ra, double lb, uint32_t rb) { return la > lb || (la == lb && ra < rb); }
 
-// the k-th largest of n floats in LDS (n >= k >= 1; room for whole float4), every thread gets it: rank by counting
-template <uint32_t THREADS>
-__device__ float kth_of(const float *v, uint32_t n, uint32_t k, float *out)
+// the k-th largest of n floats in LDS (k <= n <= kFinGroups), every thread gets it.  By one wave, bit by bit from the top: the largest key that
+// k values reach.  (Ranks by counting, a thread per value: 13 us for 256 of them; up to 64 are counted, a few less than the 32 bits.)
+__device__ __forceinline__ float kth_of(const float *v, uint32_t n, uint32_t k, float *out)
 {
-    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-        const float a = v[i];
-        uint32_t before = 0;
+    if (threadIdx.x < 64u && n <= 64u) {
+        const float mine = threadIdx.x < n ? v[threadIdx.x] : neg_inf();
+        uint32_t above = 0;
         for (uint32_t j = 0; j < n; j += 4u) {
-            const float4 b = *(const float4 *)(v + j);
-            const float c[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (uint32_t x = 0; x < 4u; ++x)
-                before += j + x < n && (c[x] > a || (c[x] == a && j + x < i)) ? 1u : 0u;
+            const float4 o = *(const float4 *)(v + j);
+            above += (o.x > mine ? 1u : 0u) + (j + 1u < n && o.y > mine ? 1u : 0u) + (j + 2u < n && o.z > mine ? 1u : 0u) +
+                     (j + 3u < n && o.w > mine ? 1u : 0u);
         }
-        if (before == k - 1u)
-            *out = a;
+        const float r = -wave_max(above < k ? -mine : neg_inf()); // (beyond n: at least n >= k are above, or all are -inf)
+        if (threadIdx.x == 0)
+            *out = r;
+    } else if (threadIdx.x < 64u) {
+        constexpr uint32_t kPer = kFinGroups / 64u;
+        uint32_t key[kPer]; // ordered as the floats are; 0: none
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; ++i) {
+            const uint32_t bits = __float_as_uint(v[min(i * 64u + threadIdx.x, n - 1u)]);
+            key[i] = i * 64u + threadIdx.x < n ? bits ^ ((bits >> 31) ? 0xffffffffu : 0x80000000u) : 0u;
+        }
+        uint32_t found = 0;
+#pragma unroll 1
+        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+            uint32_t reach = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i)
+                reach += (uint32_t)__popcll(__ballot(key[i] >= (found | bit)));
+            if (n > 256u) {
+#pragma unroll
+                for (uint32_t i = 4; i < kPer; ++i)
+                    reach += (uint32_t)__popcll(__ballot(key[i] >= (found | bit)));
+            }
+            if (reach >= k)
+                found |= bit;
+        }
+        if (threadIdx.x == 0)
+            *out = __uint_as_float(found ^ ((found >> 31) ? 0x80000000u : 0xffffffffu));
     }
     __syncthreads();
     const float r = *out;
@@ -230,9 +271,9 @@ __device__ float kth_of(const float *v, uint32_t n, uint32_t k, float *out)
     return r;
 }
 
-// the k first of n candidates by (logit descending, row ascending) -> best[0 .. min(n, k))
+// the k first of n candidates by (logit descending, row ascending) -> best[0 .. min(n, k)); rank: room for n
 template <uint32_t THREADS>
-__device__ void order_candidates(const FinCand *cand, uint32_t n, uint32_t k, FinCand *best)
+__device__ void order_candidates(const FinCand *cand, uint32_t n, uint32_t k, FinCand *best, uint32_t *rank)
 {
     if (n <= 64u) { // one wave, from registers
         if (threadIdx.x < 64u) {
@@ -248,15 +289,26 @@ __device__ void order_candidates(const FinCand *cand, uint32_t n, uint32_t k, Fi
         __syncthreads();
         return;
     }
-    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+    // each candidate's rank, counted by as many threads as there are for it
+    const uint32_t parts = max(THREADS / n, 1u);
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS)
+        rank[i] = 0;
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < n * parts; t += THREADS) {
+        const uint32_t i = t % n, part = t / n;
         const double l = cand[i].l;
         const uint32_t r = cand[i].row;
         uint32_t before = 0;
-        for (uint32_t j = 0; j < n; ++j)
+#pragma unroll 4
+        for (uint32_t j = part; j < n; j += parts)
             before += cand_before(cand[j].l, cand[j].row, l, r) ? 1u : 0u;
-        if (before < k)
-            best[before].l = l, best[before].row = r;
+        if (before)
+            atomicAdd(&rank[i], before);
     }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS)
+        if (rank[i] < k)
+            best[rank[i]].l = cand[i].l, best[rank[i]].row = cand[i].row;
     __syncthreads();
 }
 
@@ -313,7 +365,7 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
     __shared__ double red[2][WAVES];
     __shared__ float lm[WAVES][64];                // the threads' maxima
     __shared__ __align__(16) float lv[kFinGroups]; // maxima of the candidate groups (first, of the buckets)
-    __shared__ uint32_t lg[kFinGroups];            // candidate groups
+    __shared__ uint32_t lg[kFinGroups];            // candidate groups; then candidates' ranks
     __shared__ uint32_t lu[kFinGroups];            // candidate units; then candidate rows
     __shared__ FinCand cand[kFinRows + VFSX_LOG_PROBS_MAX_K];
     __shared__ FinCand best[VFSX_LOG_PROBS_MAX_K];
@@ -400,7 +452,7 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
                 lv[tid] = v;
             }
             __syncthreads();
-            first = kth_of<THREADS>(lv, kBuckets, k, &kth);
+            first = kth_of(lv, kBuckets, k, &kth);
         }
         float thr = below(first);
         // units above it -> pieces -> groups
@@ -451,7 +503,7 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
         if (whole) {
             const uint32_t n = n_lg;
             if (n > k) // the k-th largest group maximum: a closer bound
-                thr = fmaxf(thr, below(kth_of<THREADS>(lv, n, k, &kth)));
+                thr = fmaxf(thr, below(kth_of(lv, n, k, &kth)));
             // their rows: in f32 first, then those that are left in f64, and the given rows beside them
             const float fac = (float)(st.cosine ? 1.0 / (qs.norm[qi] * st.divide) : 1.0 / st.divide);
             for (uint32_t i = wave; i < n; i += WAVES) {
@@ -480,7 +532,7 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
                 __syncthreads();
             }
             if (whole) {
-                order_candidates<THREADS>(cand, n_rows, k, best);
+                order_candidates<THREADS>(cand, n_rows, k, best, lg);
                 have = min(n_rows, k);
             }
         }
@@ -504,7 +556,7 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
                     const uint32_t group = g0 + (uint32_t)__ffsll((unsigned long long)todo) - 1u;
                     for (uint32_t j = 0; j < kGroupRows; ++j) {
                         const uint32_t r = group * kGroupRows + j;
-                        const double l = row_logit<SRC>(st, qs, qi, r);
+                        const double l = r < st.n_rows ? row_logit<SRC>(st, qs, qi, r) : -__builtin_inf();
                         if (lane == 0 && l != -__builtin_inf() && (have < k || cand_before(l, r, best[k - 1u].l, best[k - 1u].row))) {
                             const uint32_t at = atomicAdd(&n_cand, 1u); // at most 64 groups of 8 rows
                             cand[at].l = l, cand[at].row = r;
@@ -518,7 +570,7 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
                 for (uint32_t i = tid; i < have; i += THREADS)
                     cand[fresh + i] = best[i];
                 __syncthreads();
-                order_candidates<THREADS>(cand, fresh + have, k, best);
+                order_candidates<THREADS>(cand, fresh + have, k, best, lg);
                 have = min(fresh + have, k);
             }
         }
@@ -543,6 +595,7 @@ __global__ __launch_bounds__(THREADS) void prob_finish_kernel(ProbStore st, Prob
                 bool first = true; // of its group
                 for (uint32_t i = 0; i < j0; ++i)
                     first = first && best[i].row / kGroupRows != group;
+#pragma unroll 4
                 for (uint32_t i = 0; i < 64u && j0 + i + 1u < have; ++i) // (uniform)
                     first = first && !(i < lane && (uint32_t)__builtin_amdgcn_readlane((int)group, (int)i) == group);
                 if (first) {

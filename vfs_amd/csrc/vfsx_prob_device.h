@@ -80,16 +80,20 @@ __device__ __forceinline__ T chunk_dot(uint4 v, const float *__restrict__ q, T a
     return acc;
 }
 
-// the same for chunk c when it is a row's last and not whole: the query has nothing beyond dim
+// the same for chunk c when it is a row's last and not whole: the query has nothing beyond dim, and the row zeros.  (The query's last element
+// again, not a branch: sixteen loads that wait for each other otherwise.)
 template <int SRC, typename T>
 __device__ __forceinline__ T chunk_dot_part(uint4 v, const float *__restrict__ q, uint32_t c, uint32_t dim, T acc)
 {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     constexpr uint32_t per = SRC == kProbI8 ? 16u : 4u;
+    float a[per];
 #pragma unroll
     for (uint32_t i = 0; i < per; ++i)
-        if (c * per + i < dim)
-            acc = fma_of(SRC == kProbI8 ? (T)i8_at(w[i >> 2], i & 3) : (T)__uint_as_float(w[i & 3]), (T)q[c * per + i], acc);
+        a[i] = q[min(c * per + i, dim - 1u)];
+#pragma unroll
+    for (uint32_t i = 0; i < per; ++i)
+        acc = fma_of(SRC == kProbI8 ? (T)i8_at(w[i >> 2], i & 3) : (T)__uint_as_float(w[i & 3]), (T)a[i], acc);
     return acc;
 }
 
