@@ -7,8 +7,7 @@
 //   m = max l,  s = sum exp(l - m),  t = sum exp(l - m) (l - m)
 // and for each GROUP of 8 rows its maximum.  Second pass, one workgroup per query: with M = max m
 //   S = sum s e^(m-M),  U = sum (t + (m - M) s) e^(m-M),   lse = M + log S,   H = log S - U / S
-// First-pass logits are f32 (f32-grade
-// products, f32 exponentials); the joined sums are f64.
+// First-pass logits are f32 (f32-grade products, f32 exponentials); the joined sums are f64.
 //
 // Most probable rows: first-pass logits are off by at most eps (below), so a row of the true top k lies in a group whose maximum is
 // at least (k-th largest group maximum) - 2 eps.  The rows of those groups, about k of them, are computed again in f64 and ordered by
@@ -117,6 +116,7 @@ __global__ __launch_bounds__(256) void prob_queries_kernel(ProbStore st, const f
 // What is left per query is small (16 bytes per 64 rows, 4 per 8) but serial: joined sums, then a bound, then the few groups above
 // it, then the few rows of those.  It is bound by latency for one query -- hence 1024 threads then, and loads in flight side by side -- and
 // by what the candidate groups read for a batch: k groups or a few more, each 8 rows = 128 bytes, one cache line, of every chunk.
+// One query, 2153 x 16: 10..12 us, 1M x 768: 19..25; 37 queries, top 20, 32749 x 777: 28; 4096 queries, top 10, 100000 x 768: 296 us, 2.1 GB.
 constexpr uint32_t kFinGroups = 1024; // candidate groups kept at once
 constexpr uint32_t kFinRows = 1024;   // candidate rows kept at once
 constexpr uint32_t kBuckets = 256;    // maxima that the first bound of many rows is taken from

@@ -1,4 +1,4 @@
-// vfsx_prob_device.h -- device code that vfsx_prob.hip and vfsx_f8.hip share.
+// vfsx_prob_device.h -- device code that vfsx_prob.hip, vfsx_stream.hip, vfsx_few.hip and vfsx_f8.hip share.
 #pragma once
 
 #include <hip/hip_runtime.h>
