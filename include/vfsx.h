@@ -472,8 +472,8 @@ typedef enum vfsx_source { VFSX_SOURCE_ROWS = 0, VFSX_SOURCE_F8 = 1 } vfsx_sourc
  * log p over all shards is log p + lse - log sum_shards exp(lse).
  * Calls on one corpus share its workspaces, as searches do (see vfsx_search_device).  Under HIP graph capture the call makes no
  * allocation: call vfsx_reserve_log_probs with at least these sizes first (VFSX_ERR_MEMTABLE otherwise); memory a captured
- * call used stays until the corpus is destroyed, the graph is valid until rows are appended, and a replay counts as a call: replays
- * and calls on one corpus must not overlap.
+ * call used stays until the corpus is destroyed, the graph is valid until rows are appended or the 8-bit copy is switched off,
+ * and a replay counts as a call: replays and calls on one corpus must not overlap.
  */
 int vfsx_log_probs_device(vfsx_corpus *c, const float *d_queries, uint32_t nq, int similarity, double temperature, int source,
                           const float *d_bias, const uint64_t *d_rows, uint32_t n_given, uint32_t k, float *d_log_probs,

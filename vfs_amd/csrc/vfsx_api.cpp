@@ -2034,7 +2034,8 @@ struct ProbCarve {
     size_t fac, eps, norm, operand, q8_exp, pieces, groups, units, bytes;
 };
 constexpr uint32_t kProbQueryTile = 128; // queries of one workgroup of the first pass, at most
-constexpr size_t kProbRoundBytes = 512u << 20; // statistics of one round of queries
+constexpr size_t kProbRoundBytes = 512u << 20; // statistics of one round of queries; operands of one
+constexpr size_t kProbTileBytes = 8ull << 30;  // what a round of one tile may take beyond that (a round reads the whole store)
 
 ProbCarve prob_carve(const vfsx_corpus *c, uint32_t nq, bool f8, bool statistics)
 {
@@ -2042,9 +2043,16 @@ ProbCarve prob_carve(const vfsx_corpus *c, uint32_t nq, bool f8, bool statistics
     const uint64_t n_pieces = (c->n_rows + vfsx::kPieceRows - 1u) / vfsx::kPieceRows;
     const uint64_t n_units = vfsx::prob_units(n_pieces);
     const uint64_t per_q = n_pieces * (sizeof(float4) + vfsx::kGroupsPerPiece * sizeof(float)) + n_units * sizeof(vfsx::ProbUnit);
+    const uint64_t operand_q = (f8 ? 2u : 4u) * (uint64_t)vfsx::query_elems(c->dim); // bf16, or f16 pairs
     uint64_t round = 32768;
-    if (statistics && per_q)
-        round = std::min<uint64_t>(round, std::max<uint64_t>(kProbQueryTile, kProbRoundBytes / per_q / kProbQueryTile * kProbQueryTile));
+    auto limit = [&](uint64_t bytes) { // whole tiles of kProbRoundBytes, or one, or what kProbTileBytes hold of it
+        if (bytes) {
+            const uint64_t tiles = kProbRoundBytes / bytes / kProbQueryTile;
+            round = std::min<uint64_t>(round, tiles ? tiles * kProbQueryTile : std::max<uint64_t>(1, std::min<uint64_t>(kProbQueryTile, kProbTileBytes / bytes)));
+        }
+    };
+    limit(statistics ? per_q : 0);
+    limit(operand_q);
     w.round = (uint32_t)std::min<uint64_t>(round, nq);
     w.pad = (w.round + kProbQueryTile - 1u) / kProbQueryTile * kProbQueryTile;
     size_t at = 0;
@@ -2056,7 +2064,7 @@ ProbCarve prob_carve(const vfsx_corpus *c, uint32_t nq, bool f8, bool statistics
     w.norm = take(w.pad * sizeof(double));
     w.fac = take(w.pad * sizeof(float));
     w.eps = take(w.pad * sizeof(float));
-    w.operand = take((size_t)w.pad * (f8 ? 2u : 4u) * vfsx::query_elems(c->dim)); // bf16, or f16 pairs
+    w.operand = take((size_t)w.pad * operand_q);
     w.q8_exp = take(f8 ? (size_t)w.pad * vfsx::f8_exp_words(c->dim) * 4u : 0);
     w.pieces = take(statistics ? (size_t)w.round * n_pieces * sizeof(float4) : 0);
     w.groups = take(statistics ? (size_t)w.round * n_pieces * vfsx::kGroupsPerPiece * sizeof(float) : 0);
