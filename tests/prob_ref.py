@@ -128,3 +128,24 @@ def compare(got, want, l, bound):
         assert np.array_equal(got.top_rows.astype(np.int64)[:, :w.shape[1]], w), (got.top_rows.astype(np.int64)[:, :w.shape[1]], w)
         assert (got.top_rows[:, w.shape[1]:] == np.uint64(2**64 - 1)).all()
         assert np.array_equal(got.top_count, want["top_count"])
+
+
+def refused(call):
+    """The code of the VfsxError that call() raises, or None.  The exception is not kept: its traceback would keep the caller's stores and
+    graphs until a garbage collection, wherever that comes."""
+    import vfs_amd
+    try:
+        call()
+    except vfs_amd.VfsxError as e:
+        return e.code
+    return None
+
+
+def no_collection():
+    """For tests that capture graphs: garbage of earlier tests goes first, and none is collected in between.  (A graph that is destroyed
+    inside a capture synchronizes the device, which the capture forbids: torch's destructor then ends the process.)"""
+    import gc
+    gc.collect()
+    gc.disable()
+    yield
+    gc.enable()

@@ -7,6 +7,7 @@ from vfs_amd import _lib
 from tests import prob_ref as ref
 
 pytestmark = pytest.mark.gpu
+no_collection = pytest.fixture(ref.no_collection)
 
 
 def make(n, d, rng):
@@ -94,6 +95,25 @@ def test_scores_against_definition(size, similarity, dtype):
         assert np.array_equal(c.scores_f8(q, similarity), got[:nq, :n].astype(np.float32))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,d,nq", [(500, 130, 40), (9008, 72, 600), (300, 40, 3)])
+def test_scores_into_any_address(n, d, nq, dtype):
+    """Output rows that begin at any element, not at 16 bytes: the same scores, and nothing else touched."""
+    import torch
+    rng = np.random.default_rng(n)
+    rows, q = make(n, d, rng), torch.from_numpy(rng.standard_normal((nq, d)).astype(np.float32)).cuda()
+    c = f8_corpus(rows)
+    t, stream = torch.float32 if dtype == "f32" else torch.bfloat16, torch.cuda.current_stream().cuda_stream
+    want = torch.empty((nq, n), device="cuda", dtype=t)
+    c.scores_f8_device(q.data_ptr(), nq, want.data_ptr(), dtype=dtype, stream=stream)
+    for offset, ld in ((1, n), (3, n + 8), (0, n + 1)):
+        flat = torch.full((offset + nq * ld + 9,), 7.0, device="cuda", dtype=t)
+        c.scores_f8_device(q.data_ptr(), nq, flat.data_ptr() + offset * flat.element_size(), ld=ld, dtype=dtype, stream=stream)
+        got = flat[offset:offset + nq * ld].view(nq, ld)
+        assert torch.equal(got[:, :n], want) and (got[:, n:] == 7).all()
+        assert (flat[:offset] == 7).all() and (flat[offset + nq * ld:] == 7).all()
+
+
 def test_scores_of_odd_values():
     rng = np.random.default_rng(1)
     rows, q = make(100, 140, rng), rng.standard_normal((34, 140)).astype(np.float32)
@@ -149,9 +169,8 @@ def test_copy_follows_appends_and_can_be_switched():
     assert c.storage_info()["device_bytes"] < before
     for call in (lambda: c.scores_f8(q), lambda: c.get_rows_f8([0]), lambda: c.log_probs(q, source="f8"), lambda: c.reserve_scores_f8(1),
                  lambda: c.reserve_log_probs(1, source="f8")):
-        with pytest.raises(vfs_amd.VfsxError) as e:
-            call()
-        assert e.value.code == _lib.ERR_INVALID_VECTOR and "enable_f8" in str(e.value)
+        assert ref.refused(call) == _lib.ERR_INVALID_VECTOR
+        assert b"enable_f8" in c._lib.vfsx_last_error()
     c.enable_f8()
     assert np.array_equal(c.scores_f8(q), f8_corpus(rows).scores_f8(q))
 
@@ -177,7 +196,7 @@ def test_refusals():
     assert c.scores_f8(q).shape == (2, 20)
 
 
-def test_captured_graph():
+def test_captured_graph(no_collection):
     import torch
     rng = np.random.default_rng(5)
     c = f8_corpus(make(700, 300, rng))
