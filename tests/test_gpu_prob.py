@@ -409,7 +409,7 @@ def test_current_device_is_left_alone():
 
 
 def test_several_rounds_of_queries():
-    """Queries whose statistics do not fit one round: 512 MiB hold 256-query rounds here."""
+    """Queries whose statistics do not fit one round: 512 MiB hold 128 of them here."""
     rng = np.random.default_rng(14)
     n, nq = 5_000_000, 300
     c = vfs_amd.Corpus(4, capacity_rows=n)
@@ -417,7 +417,7 @@ def test_several_rounds_of_queries():
     c.append(rows)
     q = rng.standard_normal((nq, 4)).astype(np.float32)
     got = c.log_probs(q, np.arange(nq)[:, None], 3)
-    for i in (0, 1, 255, 256, 257, 299):
+    for i in (0, 1, 127, 128, 129, 255, 256, 257, 299):
         l = ref.logits(rows, q[i:i + 1])
         one = type(got)(*(a[i:i + 1] for a in got))
         ref.compare(one, ref.softmax_of(l, np.array([[i]]), 3), l, ref.logit_bound(rows, q[i:i + 1]))
