@@ -442,7 +442,9 @@ __global__ __launch_bounds__(WAVES * QW * 64, (Step<SRC, NT, WAVES, QW>::kWavesP
             const float inv = st.cosine && my < st.n_rows ? st.row_inv[my] : 1.0f;
             row_mul[wave][lane] = inv < 0.0f ? __builtin_nanf("") : inv;
             const uint32_t left = active ? st.n_rows - rb * 64u : 0u; // rows of this block
-            const bool whole = out.aligned && left >= 64u;
+            // bf16 whose 16 scores of a lane are 32 aligned bytes: as they are (131072 x 256, 1024 queries: 128 us, turned 166; f32, 243368 x 159,
+            // 281 queries: 116, turned 97)
+            const bool whole = EPI == kScoresBf16 && out.aligned && left >= 64u;
 #pragma unroll
             for (uint32_t nt = 0; nt < NT; ++nt) {
                 const uint32_t qi = q0 + nt * 32u;
@@ -467,9 +469,8 @@ __global__ __launch_bounds__(WAVES * QW * 64, (Step<SRC, NT, WAVES, QW>::kWavesP
                             }
                         }
                     } else {
-                        // Rows of the output that begin anywhere, or end here: a score at a time, but 32 neighbours of two queries by one
-                        // instruction, turned through LDS (a lane's own 16 scores: 64 lines an instruction; 37 queries, 32749 rows: 17.7 us,
-                        // turned 12.7).
+                        // A score at a time, but 32 neighbours of two queries by one instruction, turned through LDS, wherever the output's rows
+                        // begin or end (a lane's own 16 scores: 64 lines an instruction; f32, 32749 x 777, 37 queries: 17.7 us, turned 12.7).
 #pragma unroll
                         for (uint32_t i = 0; i < sizeof(T); ++i)
                             __builtin_memcpy(__builtin_assume_aligned((char *)&turn[wave][r32 * kTurnPitch + h * 16u] + 16u * i, 16),
